@@ -96,6 +96,9 @@ _SIZES = {DataType.kBool: 1, DataType.kFloat8E4M3FN: 1, DataType.kFloat8E5M2: 1,
           DataType.kFloat64: 8, DataType.kInt64: 8, DataType.kUInt64: 8}
 
 
+_INT32_MAX = 2 ** 31 - 1
+
+
 def data_type_size(dtype: DataType) -> int:
     return _SIZES.get(DataType(dtype), 0)
 
@@ -223,6 +226,9 @@ class OperationKind(enum.IntEnum):
     kGgufMatVec = 0x102
     kRandomBits = 0x103
     kCategorical = 0x104
+    kAttention = 0x105
+    kPagedAttention = 0x106
+    kPagedAppend = 0x107
 
 
 class UnaryKind(enum.IntEnum):
@@ -506,6 +512,42 @@ class Categorical:
     return_log_probability: bool = False
 
 
+@dataclass(frozen=True)
+class Attention:
+    """Softmax attention of whole sequences.  Inputs (queries, keys, values [, marks]): batched [B, R, Hq, D] against
+    [B, N, H, D], marks Int32 [B] valid keys; or packed [T, Hq, D] against [T, H, D], marks Int32 [S + 1] the rows where
+    sequences begin and the last one ends (rows of none are left as they were); rank 3 without marks is one sequence.
+    Batched queries stand at positions N - R + i.  Causal queries at p see keys j <= p, with a window those with
+    j > p - window or j < sinks.  Outputs: the queries' shape and type and, when asked, Float32 logarithms of the rows'
+    sums of exp(scale * product).  A row that sees nothing is zeros, its logarithm -inf."""
+    scale: float = 1.0
+    causal: bool = True
+    window: int = 0
+    sinks: int = 0
+    return_log_sum: bool = False
+
+
+@dataclass(frozen=True)
+class PagedAttention:
+    """The newest tokens of each sequence against a paged cache.  Inputs (queries [B, R, Hq, D] or [B, Hq, D], cache
+    [P, 2, H, page, D] of their type or Float8E4M3FN, pages Int32 [B, M], lengths Int32 [B] that count the new tokens).
+    Query i stands at position length - R + i; a page outside [0, P) holds no keys.  Outputs as Attention's."""
+    scale: float = 1.0
+    window: int = 0
+    sinks: int = 0
+    return_log_sum: bool = False
+
+
+@dataclass(frozen=True)
+class PagedAppend:
+    """Inputs (keys, values [T, H, D], Int32 [T] slots): rows written to their slots (page * page_size + place) of the
+    output, a cache [pages, 2, H, page_size, D] of `cache_type` (the keys' type or Float8E4M3FN), whose other rows stay
+    as they were.  A slot outside the cache writes nothing."""
+    pages: int = 0
+    page_size: int = 0
+    cache_type: DataType = DataType.kUnknown
+
+
 def _op_desc(operation, inputs: Sequence[TensorDesc]) -> capi.OpDescC:
     c = capi.OpDescC()
     c.abi_version = capi.ABI_VERSION
@@ -567,6 +609,16 @@ def _op_desc(operation, inputs: Sequence[TensorDesc]) -> capi.OpDescC:
         c.op, c.count = OperationKind.kRandomBits, operation.word_count
     elif isinstance(operation, Categorical):
         c.op, c.kind2 = OperationKind.kCategorical, 1 if operation.return_log_probability else 0
+    elif isinstance(operation, (Attention, PagedAttention)):
+        if not 0 <= operation.window <= _INT32_MAX or not 0 <= operation.sinks <= _INT32_MAX:
+            raise StatusError(capi.INVALID_ARGUMENT, "attention window and sinks must be counts within int32")
+        paged = isinstance(operation, PagedAttention)
+        c.op, c.kind = (OperationKind.kPagedAttention, 0) if paged else (OperationKind.kAttention, int(operation.causal))
+        c.scale, c.count, c.axis, c.kind2 = operation.scale, operation.window, operation.sinks, int(operation.return_log_sum)
+    elif isinstance(operation, PagedAppend):
+        if operation.pages < 0 or not 0 < operation.page_size <= _INT32_MAX:
+            raise StatusError(capi.INVALID_ARGUMENT, "PagedAppend requires a page count and a positive page size")
+        c.op, c.kind, c.count, c.axis = OperationKind.kPagedAppend, int(operation.cache_type), operation.pages, operation.page_size
     else:
         raise StatusError(capi.UNIMPLEMENTED, f"operation {type(operation).__name__} is not served by this provider")
     if len(inputs) > capi.MAX_INPUTS:

@@ -362,4 +362,56 @@ struct CategoricalParams {
 hipError_t launch_categorical(Elem type, const CategoricalParams &p, const void *logits, const void *identities, void *indices,
                               void *scores, void *workspace, bool vector_aligned, hipStream_t stream);
 
+// Division of numbers below 2^31 by one that is known at launch: with l = ceil(log2 d) and m = floor(2^(31 + l) / d) + 1,
+// (n * m) >> (31 + l) is n / d, since m exceeds 2^(31 + l) / d by at most 1 and n < 2^31.
+struct Divisor {
+  uint32_t divisor = 1, multiplier = 0x80000001u, shift = 31;
+  Divisor() = default;
+  explicit Divisor(uint32_t d) : divisor(d) {
+    uint32_t bits = 0;
+    while (bits < 32 && (1ull << bits) < d) ++bits;
+    shift = 31 + bits;
+    multiplier = (uint32_t)((1ull << shift) / d + 1);
+  }
+  __host__ __device__ uint32_t quotient(uint32_t n) const { return (uint32_t)(((uint64_t)n * multiplier) >> shift); }
+};
+
+// Attention of query rows over keys in memory or in a paged cache (hyle_hip.h has the rules).  Strides are in bytes.
+// marks: packed, the sequences' first rows and the end; else the valid keys of each sequence or null.
+enum class AttentionKind : uint8_t { kBatched, kPacked, kPaged };
+struct AttentionParams {
+  AttentionKind kind = AttentionKind::kBatched;
+  bool causal = true, narrow_cache = false;  // narrow: keys and values in e4m3
+  int32_t sequences = 0;
+  int32_t rows = 0;   // of each sequence; packed: of all
+  int32_t keys = 0;   // most keys of a sequence
+  int32_t queries = 0, heads = 0, shared = 1, depth = 0;  // query heads, key heads, query heads to a key head
+  int32_t window = 0, sinks = 0;
+  float scale = 1.0f;
+  int64_t q_sequence = 0, q_row = 0, q_head = 0;
+  int64_t k_sequence = 0, k_row = 0, k_head = 0;  // paged: k_sequence is the page's
+  int64_t v_sequence = 0, v_row = 0, v_head = 0;
+  int64_t value_offset = 0;                       // paged: from the keys to the values
+  int32_t pages = 0, columns = 0;
+  int64_t table_row = 0;  // entries
+  Divisor page;
+};
+struct AttentionBuffers {
+  const void *query = nullptr, *key = nullptr, *value = nullptr;
+  const int32_t *table = nullptr, *marks = nullptr;
+  void *out = nullptr;
+  float *logs = nullptr;
+};
+hipError_t launch_attention_general(Elem type, const AttentionParams &p, const AttentionBuffers &b, hipStream_t stream);
+
+// PagedAppend: rows of [tokens, heads, depth] keys and values to their slots of a dense cache.
+struct AppendParams {
+  uint32_t tokens = 0, heads = 0, depth = 0, pages = 0;
+  bool narrow_cache = false;
+  int64_t k_token = 0, k_head = 0, v_token = 0, v_head = 0;  // bytes
+  Divisor page;
+};
+hipError_t launch_paged_append(Elem type, const AppendParams &p, const void *keys, const void *values, const int32_t *slots,
+                               void *cache, bool vector_aligned, hipStream_t stream);
+
 }  // namespace hyle_hip

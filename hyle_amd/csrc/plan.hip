@@ -284,6 +284,79 @@ hyle_hip_status expect_gguf_weight(const Desc &w) {
   return HYLE_HIP_OK;
 }
 
+// Attention and PagedAttention (hyle_hip.h has the operands' shapes)
+hyle_hip_status infer_attention(const hyle_hip_op_desc &r, Desc *outs, uint32_t *out_count) {
+  const bool paged = r.op == HYLE_HIP_OP_PAGED_ATTENTION;
+  const Desc *in = r.inputs;
+  hyle_hip_status s;
+  if ((s = paged ? expect_inputs(r, 4, 4) : expect_inputs(r, 3, 4)) != HYLE_HIP_OK) return s;
+  const Desc &query = in[0];
+  if (!is_floating(query.dtype) || query.rank < 3 || query.rank > 4)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "attention requires floating queries [.., rows, heads, depth] of rank 3 or 4");
+  const int64_t query_heads = query.dims[query.rank - 2], depth = query.dims[query.rank - 1];
+  int64_t heads;
+  if (paged) {
+    const Desc &cache = in[1], &table = in[2], &lengths = in[3];
+    if (cache.rank != 5 || cache.dims[1] != 2 || cache.dims[4] != depth)
+      return fail(HYLE_HIP_INVALID_ARGUMENT, "paged attention requires a cache [pages, 2, heads, page, depth] of the queries' depth");
+    if (cache.dtype != query.dtype && cache.dtype != HYLE_HIP_DTYPE_F8_E4M3FN)
+      return fail(HYLE_HIP_INVALID_ARGUMENT, "paged attention requires a cache of the queries' type or float8 e4m3");
+    if (table.dtype != HYLE_HIP_DTYPE_I32 || table.rank != 2 || lengths.dtype != HYLE_HIP_DTYPE_I32 || lengths.rank != 1 ||
+        table.dims[0] != query.dims[0] || lengths.dims[0] != query.dims[0])
+      return fail(HYLE_HIP_INVALID_ARGUMENT, "paged attention requires i32 pages [sequences, columns] and i32 lengths [sequences]");
+    heads = cache.dims[2];
+  } else {
+    const int rank = query.rank;
+    if (r.kind > 1) return fail(HYLE_HIP_INVALID_ARGUMENT, "attention causality must be 0 or 1");
+    for (int i = 1; i < 3; ++i) {
+      if (in[i].dtype != query.dtype || in[i].rank != rank || in[i].dims[rank - 1] != depth)
+        return fail(HYLE_HIP_INVALID_ARGUMENT, "attention requires keys and values of the queries' type, rank and depth");
+      if (rank == 4 && in[i].dims[0] != query.dims[0])
+        return fail(HYLE_HIP_INVALID_ARGUMENT, "attention requires keys and values of the queries' batch");
+    }
+    for (int a = 0; a < rank; ++a)
+      if (in[1].dims[a] != in[2].dims[a])
+        return fail(HYLE_HIP_INVALID_ARGUMENT, "attention requires keys and values of one shape");
+    if (r.input_count == 4) {
+      if (in[3].dtype != HYLE_HIP_DTYPE_I32 || in[3].rank != 1 || (rank == 4 ? in[3].dims[0] != query.dims[0] : in[3].dims[0] == 0))
+        return fail(HYLE_HIP_INVALID_ARGUMENT, "attention requires i32 marks: [batch] valid keys, or [sequences + 1] rows of a packed batch");
+      if (rank == 3 && in[1].dims[0] != query.dims[0])
+        return fail(HYLE_HIP_INVALID_ARGUMENT, "packed attention requires as many keys as queries");
+    }
+    heads = in[1].dims[rank - 2];
+  }
+  if (heads <= 0 || depth <= 0 || query_heads % heads != 0)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "attention requires a positive depth and query heads that are a multiple of the key heads");
+  if (!std::isfinite(r.scale)) return fail(HYLE_HIP_INVALID_ARGUMENT, "attention scale must be finite");
+  if (r.count > (uint64_t)std::numeric_limits<int32_t>::max() || r.axis < 0)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "attention window and sinks must be counts within int32");
+  if ((r.count != 0 && !paged && r.kind == 0) || (r.axis != 0 && r.count == 0))
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "an attention window needs causal attention, and sinks a window");
+  if (r.kind2 > 1) return fail(HYLE_HIP_INVALID_ARGUMENT, "attention's choice of logarithms must be 0 or 1");
+  if ((s = make_dense(query.dtype, query.dims, query.rank, &outs[0])) != HYLE_HIP_OK) return s;
+  if (r.kind2 == 0) return HYLE_HIP_OK;
+  *out_count = 2;
+  return make_dense(HYLE_HIP_DTYPE_F32, query.dims, query.rank - 1, &outs[1]);
+}
+
+hyle_hip_status infer_paged_append(const hyle_hip_op_desc &r, Desc *outs) {
+  const Desc *in = r.inputs;
+  hyle_hip_status s;
+  if ((s = expect_inputs(r, 3, 3)) != HYLE_HIP_OK) return s;
+  const Desc &keys = in[0], &values = in[1], &slots = in[2];
+  if (!is_floating(keys.dtype) || values.dtype != keys.dtype || keys.rank != 3 || values.rank != 3 ||
+      keys.dims[0] != values.dims[0] || keys.dims[1] != values.dims[1] || keys.dims[2] != values.dims[2])
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedAppend requires floating keys and values [tokens, heads, depth] of one type and shape");
+  if (slots.dtype != HYLE_HIP_DTYPE_I32 || slots.rank != 1 || slots.dims[0] != keys.dims[0])
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedAppend requires i32 slots [tokens]");
+  if (r.kind != keys.dtype && r.kind != HYLE_HIP_DTYPE_F8_E4M3FN)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedAppend requires a cache of the keys' type or float8 e4m3");
+  if (r.axis <= 0 || r.count > (uint64_t)std::numeric_limits<int32_t>::max() / (uint64_t)r.axis)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedAppend requires a positive page size and slots within int32");
+  const int64_t dims[5] = {(int64_t)r.count, 2, keys.dims[1], r.axis, keys.dims[2]};
+  return make_dense((uint8_t)r.kind, dims, 5, &outs[0]);
+}
+
 hyle_hip_status infer(const hyle_hip_op_desc &r, Desc *outs, uint32_t *out_count) {
   if (r.abi_version != HYLE_HIP_ABI_VERSION)
     return fail(HYLE_HIP_INVALID_ARGUMENT, "hyle_hip_op_desc ABI version %u is not %u", r.abi_version,
@@ -616,6 +689,9 @@ hyle_hip_status infer(const hyle_hip_op_desc &r, Desc *outs, uint32_t *out_count
       dims[rank++] = in[0].dims[1];
       return make_dense(in[1].dtype, dims, rank, &outs[0]);
     }
+    case HYLE_HIP_OP_ATTENTION:
+    case HYLE_HIP_OP_PAGED_ATTENTION: return infer_attention(r, outs, out_count);
+    case HYLE_HIP_OP_PAGED_APPEND: return infer_paged_append(r, outs);
     default:
       return fail(HYLE_HIP_UNIMPLEMENTED, "operation kind %u is not served by this provider", r.op);
   }
@@ -645,6 +721,8 @@ enum class Route : uint8_t {
   kRandomBits,
   kCategorical,
   kRope,
+  kAttention,
+  kPagedAppend,
 };
 
 const char *route_name(Route r) {
@@ -669,6 +747,8 @@ const char *route_name(Route r) {
     case Route::kRandomBits: return "philox-words";
     case Route::kCategorical: return "categorical-tiles";
     case Route::kRope: return "rope-rows";
+    case Route::kAttention: return "attention";
+    case Route::kPagedAppend: return "paged-append";
   }
   return "?";
 }
@@ -720,7 +800,9 @@ struct hyle_hip_plan {
   RandomBitsParams random_bits;
   CategoricalParams categorical;
   RopeParams rope;
-  // Concat and Gather take no alias and no overlap: bytes each input spans, for the launch's check
+  AttentionParams attention;
+  AppendParams append;
+  // Concat, Gather, Attention and PagedAppend take no alias and no overlap: bytes each input spans, for the launch's check
   uint64_t concat_input_bytes[HYLE_HIP_MAX_INPUTS] = {0, 0, 0, 0};
   // Cast and Copy take no alias at all (AliasPolicy::kNone, src/compute_ops/operation.cc:935-957):
   // the bytes the input and the output occupy must not overlap.
@@ -836,6 +918,118 @@ hyle_hip_status admit_gguf_rows(const Desc &w) {
     return fail(HYLE_HIP_INVALID_ARGUMENT, "GGUF row stride is shorter than a row of blocks");
   if ((uint64_t)k * (uint64_t)n > kMaxElements)
     return fail(HYLE_HIP_UNIMPLEMENTED, "GGUF weights of at most INT32_MAX values are served");
+  return HYLE_HIP_OK;
+}
+
+// The bytes from a plain tensor's first element to the end of its last (TensorDesc::required_bytes).
+uint64_t spanned_bytes(const Desc &d) {
+  if (has_zero_extent(d)) return 0;
+  uint64_t last = 0;
+  for (int a = 0; a < d.rank; ++a) last += (uint64_t)(d.dims[a] - 1) * (uint64_t)d.byte_strides[a];
+  return last + dtype_size(d.dtype);
+}
+
+// Heads are read as runs of elements: plain storage, a dense last axis, whole elements from one row to the next.
+bool has_element_rows(const Desc &d) {
+  const int64_t size = (int64_t)dtype_size(d.dtype);
+  if (is_plain(d) && has_zero_extent(d)) return true;
+  if (!is_plain(d) || (d.dims[d.rank - 1] > 1 && d.byte_strides[d.rank - 1] != size)) return false;
+  for (int a = 0; a < d.rank; ++a)
+    if (d.byte_strides[a] % size != 0) return false;
+  return true;
+}
+
+hyle_hip_status admit_attention(hyle_hip_plan *p) {
+  const hyle_hip_op_desc &r = p->request;
+  const Desc *in = r.inputs;
+  const Desc &query = in[0];
+  const bool paged = r.op == HYLE_HIP_OP_PAGED_ATTENTION;
+  if (!to_elem(query.dtype, &p->elem)) return fail(HYLE_HIP_UNIMPLEMENTED, "attention requires float32/float16/bfloat16");
+  for (uint32_t i = 0; i < (paged ? 2u : 3u); ++i)
+    if (!has_element_rows(in[i]))
+      return fail(HYLE_HIP_UNIMPLEMENTED, "attention requires plain operands with a dense last axis and whole elements to a stride");
+  for (uint32_t i = paged ? 2 : 3; i < r.input_count; ++i)
+    if (!has_element_rows(in[i])) return fail(HYLE_HIP_UNIMPLEMENTED, "attention requires plain i32 marks with dense rows");
+  const int64_t most = std::numeric_limits<int32_t>::max();
+  const int64_t depth = query.dims[query.rank - 1];
+  if (depth > 256) return fail(HYLE_HIP_UNIMPLEMENTED, "attention serves depths up to 256");
+  if (p->output_elements[0] > kMaxElements) return fail(HYLE_HIP_UNIMPLEMENTED, "attention requires at most INT32_MAX query elements");
+  if (p->output_elements[0] == 0) return HYLE_HIP_OK;
+  AttentionParams &a = p->attention;
+  const bool packed = !paged && query.rank == 3 && r.input_count == 4;
+  a.kind = paged ? AttentionKind::kPaged : packed ? AttentionKind::kPacked : AttentionKind::kBatched;
+  a.causal = paged || r.kind == 1;
+  a.depth = (int32_t)depth;
+  a.queries = (int32_t)query.dims[query.rank - 2];
+  a.window = (int32_t)r.count;
+  a.sinks = r.axis;
+  a.scale = r.scale;
+  const bool batched = query.rank == 4;
+  a.q_sequence = batched || paged ? query.byte_strides[0] : 0;
+  a.q_row = batched ? query.byte_strides[1] : paged ? 0 : query.byte_strides[0];
+  a.q_head = query.byte_strides[query.rank - 2];
+  if (paged) {
+    const Desc &cache = in[1], &table = in[2];
+    a.sequences = (int32_t)query.dims[0];
+    a.rows = batched ? (int32_t)query.dims[1] : 1;
+    a.narrow_cache = cache.dtype == HYLE_HIP_DTYPE_F8_E4M3FN;
+    a.heads = (int32_t)cache.dims[2];
+    if (cache.dims[0] > most || table.dims[1] > most || (cache.dims[3] != 0 && table.dims[1] > most / cache.dims[3]))
+      return fail(HYLE_HIP_UNIMPLEMENTED, "paged attention requires pages and positions within int32");
+    a.pages = (int32_t)cache.dims[0];
+    a.columns = (int32_t)table.dims[1];
+    a.table_row = table.byte_strides[0] / 4;
+    a.keys = (int32_t)(table.dims[1] * cache.dims[3]);
+    a.page = Divisor(cache.dims[3] > 0 ? (uint32_t)cache.dims[3] : 1u);
+    a.k_sequence = cache.byte_strides[0];
+    a.k_head = cache.byte_strides[2];
+    a.k_row = cache.byte_strides[3];
+    a.v_sequence = a.k_sequence, a.v_head = a.k_head, a.v_row = a.k_row;
+    a.value_offset = cache.byte_strides[1];
+  } else {
+    const Desc &key = in[1], &value = in[2];
+    const int row = batched ? 1 : 0;
+    if (key.dims[row] > most || (r.input_count == 4 && in[3].dims[0] > most))
+      return fail(HYLE_HIP_UNIMPLEMENTED, "attention requires key positions and sequences within int32");
+    a.sequences = packed ? (int32_t)(in[3].dims[0] - 1) : batched ? (int32_t)query.dims[0] : 1;
+    a.rows = (int32_t)query.dims[row];
+    a.keys = (int32_t)key.dims[row];
+    a.heads = (int32_t)key.dims[row + 1];
+    a.k_sequence = batched ? key.byte_strides[0] : 0;
+    a.k_row = key.byte_strides[row];
+    a.k_head = key.byte_strides[row + 1];
+    a.v_sequence = batched ? value.byte_strides[0] : 0;
+    a.v_row = value.byte_strides[row];
+    a.v_head = value.byte_strides[row + 1];
+    if (packed && a.sequences == 0) return HYLE_HIP_OK;  // every row is behind the last sequence
+  }
+  a.shared = a.queries / a.heads;
+  for (uint32_t i = 0; i < r.input_count; ++i) p->concat_input_bytes[i] = spanned_bytes(in[i]);
+  p->route = Route::kAttention;
+  p->dispatches = 1;
+  return HYLE_HIP_OK;
+}
+
+hyle_hip_status admit_paged_append(hyle_hip_plan *p) {
+  const Desc *in = p->request.inputs;
+  if (!to_elem(in[0].dtype, &p->elem)) return fail(HYLE_HIP_UNIMPLEMENTED, "PagedAppend requires float32/float16/bfloat16 keys and values");
+  for (int i = 0; i < 3; ++i)
+    if (!has_element_rows(in[i]))
+      return fail(HYLE_HIP_UNIMPLEMENTED, "PagedAppend requires plain operands with a dense last axis and whole elements to a stride");
+  if (p->input_elements[0] > kMaxElements / 2) return fail(HYLE_HIP_UNIMPLEMENTED, "PagedAppend requires at most INT32_MAX elements");
+  if (p->input_elements[0] == 0 || p->output_elements[0] == 0) return HYLE_HIP_OK;
+  AppendParams &a = p->append;
+  a.tokens = (uint32_t)in[0].dims[0];
+  a.heads = (uint32_t)in[0].dims[1];
+  a.depth = (uint32_t)in[0].dims[2];
+  a.pages = (uint32_t)p->request.count;
+  a.page = Divisor((uint32_t)p->request.axis);
+  a.narrow_cache = p->request.kind == HYLE_HIP_DTYPE_F8_E4M3FN;
+  a.k_token = in[0].byte_strides[0], a.k_head = in[0].byte_strides[1];
+  a.v_token = in[1].byte_strides[0], a.v_head = in[1].byte_strides[1];
+  for (int i = 0; i < 3; ++i) p->concat_input_bytes[i] = spanned_bytes(in[i]);
+  p->route = Route::kPagedAppend;
+  p->dispatches = 1;
   return HYLE_HIP_OK;
 }
 
@@ -1361,11 +1555,7 @@ hyle_hip_status admit(hyle_hip_plan *p) {
       // strided operands may sit at any byte: they are read bytewise
       if (!is_dense(in[0])) p->input_alignment[0] = 1;
       if (!g.dense_indices) p->input_alignment[1] = 1;
-      for (int i = 0; i < 2; ++i) {
-        uint64_t last = 0;  // byte offset of the last element: TensorDesc::required_bytes
-        for (int a = 0; a < in[i].rank; ++a) last += (uint64_t)(in[i].dims[a] - 1) * (uint64_t)in[i].byte_strides[a];
-        p->concat_input_bytes[i] = p->input_elements[i] == 0 ? 0 : last + dtype_size(in[i].dtype);
-      }
+      for (int i = 0; i < 2; ++i) p->concat_input_bytes[i] = spanned_bytes(in[i]);
       // Few indices (the rows a step picks for its last tokens, a decode batch's embeddings): every
       // moving block looks at all of them itself, which saves the checking dispatch.  At most 1024
       // indices, and at most 8 MiB of index reads over all blocks, counted for the narrowest units.
@@ -1395,6 +1585,9 @@ hyle_hip_status admit(hyle_hip_plan *p) {
       }
       return HYLE_HIP_OK;
     }
+    case HYLE_HIP_OP_ATTENTION:
+    case HYLE_HIP_OP_PAGED_ATTENTION: return admit_attention(p);
+    case HYLE_HIP_OP_PAGED_APPEND: return admit_paged_append(p);
     case HYLE_HIP_OP_COPY:
     case HYLE_HIP_OP_CAST: {
       // src/compute_provider_native/cast.cc:127-176,256-279 (admitted pairs, plain input, dense
@@ -1711,6 +1904,25 @@ static const char *noted_text(const char *end) {
 const char *hyle_hip_last_launch_variant(void) { return noted_text("#"); }
 const char *hyle_hip_last_launch_form(void) { return noted_text(""); }
 
+// Operations that take no alias: no byte of an output may be an input's, nor another output's.
+static hyle_hip_status refuse_overlaps(const hyle_hip_plan *plan, const void *const *inputs, void *const *outputs, const char *what) {
+  for (uint32_t o = 0; o < plan->output_count; ++o) {
+    const uintptr_t first = reinterpret_cast<uintptr_t>(outputs[o]);
+    const uint64_t bytes = plan->output_elements[o] * dtype_size(plan->outputs[o].dtype);
+    for (uint32_t i = 0; i < plan->request.input_count; ++i) {
+      const uintptr_t input = reinterpret_cast<uintptr_t>(inputs[i]);
+      if (input < first + bytes && first < input + plan->concat_input_bytes[i])
+        return fail(HYLE_HIP_INVALID_ARGUMENT, "input %u and output %u storage overlap; %s takes no alias", i, o, what);
+    }
+    for (uint32_t other = 0; other < o; ++other) {
+      const uintptr_t before = reinterpret_cast<uintptr_t>(outputs[other]);
+      if (before < first + bytes && first < before + plan->output_elements[other] * dtype_size(plan->outputs[other].dtype))
+        return fail(HYLE_HIP_INVALID_ARGUMENT, "outputs %u and %u storage overlap", other, o);
+    }
+  }
+  return HYLE_HIP_OK;
+}
+
 hyle_hip_status hyle_hip_plan_launch(const hyle_hip_plan *plan, const void *const *inputs,
                                      uint32_t input_count, void *const *outputs, uint32_t output_count,
                                      void *workspace, size_t workspace_size, void *stream_handle) {
@@ -1756,6 +1968,7 @@ hyle_hip_status hyle_hip_plan_launch(const hyle_hip_plan *plan, const void *cons
   }
   hipStream_t stream = static_cast<hipStream_t>(stream_handle);
   hipError_t err = hipSuccess;
+  hyle_hip_status s;
   switch (plan->route) {
     case Route::kNoOp: break;
     case Route::kEwFlat:
@@ -1856,6 +2069,25 @@ hyle_hip_status hyle_hip_plan_launch(const hyle_hip_plan *plan, const void *cons
     case Route::kRope:
       err = launch_rope(plan->elem, plan->rope, inputs[0], inputs[1], inputs[2], outputs[0],
                         aligned(inputs[0], 16) && aligned(outputs[0], 16), stream);
+      break;
+    case Route::kAttention: {
+      if ((s = refuse_overlaps(plan, inputs, outputs, "attention")) != HYLE_HIP_OK) return s;
+      AttentionBuffers b;
+      const bool paged = plan->attention.kind == AttentionKind::kPaged;
+      b.query = inputs[0];
+      b.key = inputs[1];
+      b.value = paged ? static_cast<const unsigned char *>(inputs[1]) + plan->attention.value_offset : inputs[2];
+      b.table = paged ? static_cast<const int32_t *>(inputs[2]) : nullptr;
+      b.marks = input_count > 3 ? static_cast<const int32_t *>(inputs[3]) : nullptr;
+      b.out = outputs[0];
+      b.logs = output_count > 1 ? static_cast<float *>(outputs[1]) : nullptr;
+      err = launch_attention_general(plan->elem, plan->attention, b, stream);
+      break;
+    }
+    case Route::kPagedAppend:
+      if ((s = refuse_overlaps(plan, inputs, outputs, "PagedAppend")) != HYLE_HIP_OK) return s;
+      err = launch_paged_append(plan->elem, plan->append, inputs[0], inputs[1], static_cast<const int32_t *>(inputs[2]), outputs[0],
+                                aligned(inputs[0], 16) && aligned(inputs[1], 16) && aligned(outputs[0], 16), stream);
       break;
     case Route::kRandomBits:
       err = launch_random_bits(plan->random_bits, inputs[0], outputs[0], stream);

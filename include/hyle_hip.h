@@ -167,7 +167,35 @@ typedef enum hyle_hip_op_kind {
    * nothing and shows as INVALID_ARGUMENT in hyle_hip_plan_device_status.  The draw is the CPU
    * provider's inverse CDF on the 52-bit uniform of the row's first Philox block; like the
    * reference's own backends it promises the distribution, not equal indices across backends. */
-  HYLE_HIP_OP_CATEGORICAL = 0x104
+  HYLE_HIP_OP_CATEGORICAL = 0x104,
+  /* Softmax attention of whole sequences (prompts, encoders).  in0 queries, in1 keys, in2 values of one type (F32 /
+   * F16 / BF16), any byte strides but a dense last axis; out0 like in0, dense.  `kind` = 1: causal, 0: not; `scale`
+   * (finite) multiplies the products of queries and keys; `count` = sliding window W in keys (0: none; needs
+   * causal), `axis` = sinks S >= 0 (needs a window); `kind2` = 1: out1 F32 of in0's shape without its last axis
+   * holds the natural logarithm of each row's sum of exp(scale * product).  The number of query heads is a multiple
+   * of the key heads, each of which serves as many query heads in a row.
+   *   Batched: queries [B, R, Hq, D], keys and values [B, N, H, D]; in3, if given, I32 [B]: the valid keys of each
+   *     sequence (clamped to [0, N]).  Query i stands at position N - R + i, key j at position j.  Rank 3
+   *     ([R, Hq, D], [N, H, D]) without in3 is one such sequence.
+   *   Packed: queries [T, Hq, D], keys and values [T, H, D], in3 I32 [S + 1]: sequence s is rows in3[s] up to
+   *     in3[s + 1] (they must not decrease; clamped to [0, T]) and its positions start at 0.  Rows of no sequence
+   *     are left as they were.
+   * A causal query at position p sees the keys j <= p, with a window those with j > p - W or j < S.  A row that
+   * sees nothing is zeros, its logarithm -inf.  Values and keys that a row does not see have no part in it, whatever
+   * they hold.  Products and sums are kept in f32; weights are rounded to the values' type for their products. */
+  HYLE_HIP_OP_ATTENTION = 0x105,
+  /* The same for the newest tokens of each sequence against a paged cache: in0 queries [B, R, Hq, D] or [B, Hq, D]
+   * (R = 1), in1 the cache [P, 2, H, page, D] (keys at 0, values at 1 of the second axis; in0's type or F8_E4M3FN,
+   * whose elements are the values themselves), in2 I32 [B, M] pages of each sequence in order, in3 I32 [B] lengths:
+   * the keys of each sequence, the new tokens' own among them (keys past M * page do not exist).  Query i stands at
+   * position in3 - R + i.  A page outside [0, P) holds no keys and is never read.  `scale`, `count`, `axis` and
+   * `kind2` as for ATTENTION; always causal.  A contiguous cache is one page per sequence. */
+  HYLE_HIP_OP_PAGED_ATTENTION = 0x106,
+  /* Keys and values of new tokens into such a cache: in0 keys, in1 values [T, H, D] of one type, in2 I32 [T] slots
+   * (page * page size + place in the page).  out0 is the cache, dense [P, 2, H, page, D]: `count` = P, `axis` = page
+   * size, `kind` = its type (in0's or F8_E4M3FN: nearest even, beyond +-448 the nearest end, NaN stays).  Only the
+   * tokens' rows are written.  A slot outside the cache writes nothing; of two tokens with one slot either stays. */
+  HYLE_HIP_OP_PAGED_APPEND = 0x107
 } hyle_hip_op_kind;
 
 /* UnaryKind (include/hyle/compute/operation.h:57-73) */
@@ -236,19 +264,22 @@ typedef struct hyle_hip_tensor_desc {
 typedef struct hyle_hip_op_desc {
   uint32_t abi_version;      /* HYLE_HIP_ABI_VERSION */
   uint32_t op;               /* hyle_hip_op_kind */
-  uint32_t kind;             /* Unary/Binary/Reduction/GatedActivation kind; Cast, Fill: output hyle_hip_dtype */
+  uint32_t kind;             /* Unary/Binary/Reduction/GatedActivation kind; Cast, Fill, PagedAppend: output hyle_hip_dtype;
+                                Attention: 1 = causal */
   uint32_t kind2;            /* BINARY_CHAIN: second BinaryKind; GATED: GatedInputKind;
                                 SOFTMAX: SoftmaxKind; GGUF_MATVEC: HYLE_HIP_ACTIVATIONS_*;
                                 GATHER: hyle_hip_index_bounds; CATEGORICAL: 1 = also log probabilities;
-                                ROPE: hyle_hip_rope_layout */
-  int32_t axis;              /* Softmax / TopK / Concat / Gather axis, RoPE sequence axis (negative counts from the end) */
+                                ROPE: hyle_hip_rope_layout; ATTENTION, PAGED_ATTENTION: 1 = also the rows' logarithms */
+  int32_t axis;              /* Softmax / TopK / Concat / Gather axis, RoPE sequence axis (negative counts from the end);
+                                Attention, PagedAttention: sinks; PagedAppend: page size */
   uint32_t mask;             /* Softmax MaskKind */
   uint32_t accumulation;     /* hyle_hip_dtype; UNKNOWN or F32 */
   uint32_t keep_dimensions;  /* Reduce */
   float epsilon;             /* RmsNorm, LayerNorm */
-  float scale;               /* Softmax */
+  float scale;               /* Softmax, Attention, PagedAttention */
   uint64_t count;            /* TopK count; Fill: the scalar's bits; Concat: the group's start on the axis;
-                                RandomBits: word_count; RoPE: rotary_dimensions */
+                                RandomBits: word_count; RoPE: rotary_dimensions; Attention, PagedAttention:
+                                window; PagedAppend: pages */
   uint32_t largest;          /* TopK: 1 = largest first, 0 = smallest first */
   uint32_t input_count;
   hyle_hip_tensor_desc inputs[HYLE_HIP_MAX_INPUTS];

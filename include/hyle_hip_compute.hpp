@@ -355,9 +355,20 @@ struct RoPE final {
 // sampling_ops::RandomBits / Categorical (include/hyle/compute/sampling_ops.h:12-75)
 struct RandomBits final { std::uint32_t word_count = 4; };
 struct Categorical final { bool return_log_probability = false; };
+// Softmax attention over whole sequences, over a paged cache, and what writes that cache (the inputs and the rules of
+// visibility stand at HYLE_HIP_OP_ATTENTION, _PAGED_ATTENTION and _PAGED_APPEND in hyle_hip.h).
+struct Attention final {
+  float scale = 1.0F;
+  bool causal = true;
+  std::uint32_t window = 0;
+  std::int32_t sinks = 0;
+  bool return_log_sum = false;
+};
+struct PagedAttention final { float scale = 1.0F; std::uint32_t window = 0; std::int32_t sinks = 0; bool return_log_sum = false; };
+struct PagedAppend final { std::size_t pages = 0; std::int32_t page_size = 0; DataType cache_type = DataType::kUnknown; };
 
 using Operation = std::variant<Copy, Fill, Select, Concat, Gather, Cast, Unary, Binary, Reduce, RmsNorm, LayerNorm, GatedActivation, Softmax, TopK, BinaryChain,
-                               Q8_0DequantSumSquares, GgufMatVec, RandomBits, Categorical, RoPE>;
+                               Q8_0DequantSumSquares, GgufMatVec, RandomBits, Categorical, RoPE, Attention, PagedAttention, PagedAppend>;
 
 namespace detail {
 inline hyle_hip_op_desc to_c(const Operation &operation, const TensorDesc *inputs, std::size_t count) noexcept {
@@ -417,6 +428,17 @@ inline hyle_hip_op_desc to_c(const Operation &operation, const TensorDesc *input
       r.op = HYLE_HIP_OP_ROPE; r.count = o.rotary_dimensions; r.axis = o.sequence_axis; r.kind2 = static_cast<std::uint32_t>(o.layout);
     }
     void operator()(const RandomBits &o) const { r.op = HYLE_HIP_OP_RANDOM_BITS; r.count = o.word_count; }
+    void operator()(const Attention &o) const {
+      r.op = HYLE_HIP_OP_ATTENTION; r.kind = o.causal ? 1u : 0u; r.scale = o.scale; r.count = o.window; r.axis = o.sinks;
+      r.kind2 = o.return_log_sum ? 1u : 0u;
+    }
+    void operator()(const PagedAttention &o) const {
+      r.op = HYLE_HIP_OP_PAGED_ATTENTION; r.scale = o.scale; r.count = o.window; r.axis = o.sinks;
+      r.kind2 = o.return_log_sum ? 1u : 0u;
+    }
+    void operator()(const PagedAppend &o) const {
+      r.op = HYLE_HIP_OP_PAGED_APPEND; r.kind = static_cast<std::uint32_t>(o.cache_type); r.count = o.pages; r.axis = o.page_size;
+    }
     void operator()(const Categorical &o) const { r.op = HYLE_HIP_OP_CATEGORICAL; r.kind2 = o.return_log_probability ? 1u : 0u; }
   };
   std::visit(Fill{r}, operation);
