@@ -402,6 +402,8 @@ struct AttentionBuffers {
   void *out = nullptr;
   float *logs = nullptr;
 };
+bool attention_tiles_serves(Elem type, const AttentionParams &p, bool vector_aligned);
+hipError_t launch_attention_tiles(Elem type, const AttentionParams &p, const AttentionBuffers &b, hipStream_t stream);
 hipError_t launch_attention_general(Elem type, const AttentionParams &p, const AttentionBuffers &b, hipStream_t stream);
 
 // PagedAppend: rows of [tokens, heads, depth] keys and values to their slots of a dense cache.

@@ -2081,7 +2081,9 @@ hyle_hip_status hyle_hip_plan_launch(const hyle_hip_plan *plan, const void *cons
       b.marks = input_count > 3 ? static_cast<const int32_t *>(inputs[3]) : nullptr;
       b.out = outputs[0];
       b.logs = output_count > 1 ? static_cast<float *>(outputs[1]) : nullptr;
-      err = launch_attention_general(plan->elem, plan->attention, b, stream);
+      const bool vectors = aligned(inputs[0], 16) && aligned(inputs[1], 16) && aligned(b.value, 16) && aligned(b.out, 16);
+      if (attention_tiles_serves(plan->elem, plan->attention, vectors)) err = launch_attention_tiles(plan->elem, plan->attention, b, stream);
+      else err = launch_attention_general(plan->elem, plan->attention, b, stream);
       break;
     }
     case Route::kPagedAppend:
