@@ -10,38 +10,11 @@
 // second product from the registers it was computed in: a lane's 8 keys of a 16-key step are 4h..4h+3 and 8+4h..8+4h+3 (h =
 // lane / 32), and the columns of V are read in that order too, for the sum over the keys does not care.
 // O is rescaled only when a maximum has grown by more than kSlack (2^8 stays exact in every type here).
-#include "attention.h"
-
-#include <type_traits>
+#include "attention_math.h"
 
 namespace hyle_hip {
 namespace {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr float kSlack = 8.0f;
-
-template <class T> __device__ __forceinline__ f32x16 product(u32x4 a, u32x4 b, f32x16 c) {
-  if constexpr (std::is_same<T, BF16>::value)
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-template <class T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (std::is_same<T, BF16>::value) return pack_bf16x2(lo, hi);
-  else {
-    const f32x2 in = {lo, hi};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(in, f16x2));
-  }
-}
-// 4 rows of 16 elements each, a lane of 16 its column: rows at `lane % 16 / 4`, 8 bytes at `lane % 4`.
-__device__ __forceinline__ uint2 read_transposed(const unsigned char *at) {
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at));
-}
 __device__ __forceinline__ float other_half_max(float v) {
   const auto both = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);
   return fmaxf(bits_f32(both[0]), bits_f32(both[1]));
@@ -185,14 +158,7 @@ __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_tiles(Attention
       if (row >= kKeys) continue;
       *reinterpret_cast<u32x4 *>(buffer + row * kKeyRow + chunk * 16) = staged_keys[i];
       *reinterpret_cast<u32x4 *>(buffer + kKeys * kKeyRow + row * kValueRow + chunk * 16) = staged_values[i];
-      if (!whole) {
-        constexpr uint32_t kExponent = std::is_same<T, BF16>::value ? 0x7F80u : 0x7C00u;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t word = staged_values[i][w];
-          found |= (uint32_t)((word & kExponent) == kExponent) | (uint32_t)(((word >> 16) & kExponent) == kExponent);
-        }
-      }
+      if (!whole) found |= no_numbers<T>(staged_values[i]);
     }
     if (found != 0) no_number = step + 1;
   };

@@ -402,6 +402,16 @@ struct AttentionBuffers {
   void *out = nullptr;
   float *logs = nullptr;
 };
+// The split over the keys: chunks that the keys are dealt to, slots of the grid, whether a second kernel joins, the workspace.
+struct AttentionSplit {
+  int target = 1, slots = 0;
+  bool joined = false;
+  size_t stats_offset = 0, workspace = 0;
+};
+AttentionSplit attention_split_of(const AttentionParams &p, int compute_units);
+bool attention_split_serves(Elem type, const AttentionParams &p, bool vector_aligned);
+hipError_t launch_attention_split(Elem type, const AttentionParams &p, const AttentionBuffers &b, const AttentionSplit &split, void *workspace,
+                                  hipStream_t stream);
 bool attention_tiles_serves(Elem type, const AttentionParams &p, bool vector_aligned);
 hipError_t launch_attention_tiles(Elem type, const AttentionParams &p, const AttentionBuffers &b, hipStream_t stream);
 hipError_t launch_attention_general(Elem type, const AttentionParams &p, const AttentionBuffers &b, hipStream_t stream);

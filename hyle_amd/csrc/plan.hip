@@ -801,6 +801,8 @@ struct hyle_hip_plan {
   CategoricalParams categorical;
   RopeParams rope;
   AttentionParams attention;
+  AttentionSplit attention_split;
+  bool attention_few_rows = false;  // the kernel that splits over the keys, where it serves the operands
   AppendParams append;
   // Concat, Gather, Attention and PagedAppend take no alias and no overlap: bytes each input spans, for the launch's check
   uint64_t concat_input_bytes[HYLE_HIP_MAX_INPUTS] = {0, 0, 0, 0};
@@ -939,7 +941,7 @@ bool has_element_rows(const Desc &d) {
   return true;
 }
 
-hyle_hip_status admit_attention(hyle_hip_plan *p) {
+hyle_hip_status admit_attention(hyle_hip_plan *p, uint32_t units) {
   const hyle_hip_op_desc &r = p->request;
   const Desc *in = r.inputs;
   const Desc &query = in[0];
@@ -950,7 +952,7 @@ hyle_hip_status admit_attention(hyle_hip_plan *p) {
       return fail(HYLE_HIP_UNIMPLEMENTED, "attention requires plain operands with a dense last axis and whole elements to a stride");
   for (uint32_t i = paged ? 2 : 3; i < r.input_count; ++i)
     if (!has_element_rows(in[i])) return fail(HYLE_HIP_UNIMPLEMENTED, "attention requires plain i32 marks with dense rows");
-  const int64_t most = std::numeric_limits<int32_t>::max();
+  const int64_t most = std::numeric_limits<int32_t>::max() - 255;  // kernels count past the last key by up to a tile
   const int64_t depth = query.dims[query.rank - 1];
   if (depth > 256) return fail(HYLE_HIP_UNIMPLEMENTED, "attention serves depths up to 256");
   if (p->output_elements[0] > kMaxElements) return fail(HYLE_HIP_UNIMPLEMENTED, "attention requires at most INT32_MAX query elements");
@@ -979,7 +981,7 @@ hyle_hip_status admit_attention(hyle_hip_plan *p) {
     a.pages = (int32_t)cache.dims[0];
     a.columns = (int32_t)table.dims[1];
     a.table_row = table.byte_strides[0] / 4;
-    a.keys = (int32_t)(table.dims[1] * cache.dims[3]);
+    a.keys = a.pages == 0 ? 0 : (int32_t)(table.dims[1] * cache.dims[3]);
     a.page = Divisor(cache.dims[3] > 0 ? (uint32_t)cache.dims[3] : 1u);
     a.k_sequence = cache.byte_strides[0];
     a.k_head = cache.byte_strides[2];
@@ -1007,6 +1009,14 @@ hyle_hip_status admit_attention(hyle_hip_plan *p) {
   for (uint32_t i = 0; i < r.input_count; ++i) p->concat_input_bytes[i] = spanned_bytes(in[i]);
   p->route = Route::kAttention;
   p->dispatches = 1;
+  // few rows to a key head leave the tiles of 128 rows empty and the device too, so the keys are split instead
+  p->attention_few_rows = paged || (!packed && (int64_t)a.rows * a.shared <= 64);
+  if (p->attention_few_rows && attention_split_serves(p->elem, a, true)) {
+    p->attention_split = attention_split_of(a, (int)units);
+    p->workspace_size = p->attention_split.workspace;
+    p->workspace_alignment = p->workspace_size != 0 ? 256 : 1;
+    p->dispatches = p->attention_split.joined ? 2 : 1;
+  }
   return HYLE_HIP_OK;
 }
 
@@ -1586,7 +1596,7 @@ hyle_hip_status admit(hyle_hip_plan *p) {
       return HYLE_HIP_OK;
     }
     case HYLE_HIP_OP_ATTENTION:
-    case HYLE_HIP_OP_PAGED_ATTENTION: return admit_attention(p);
+    case HYLE_HIP_OP_PAGED_ATTENTION: return admit_attention(p, units);
     case HYLE_HIP_OP_PAGED_APPEND: return admit_paged_append(p);
     case HYLE_HIP_OP_COPY:
     case HYLE_HIP_OP_CAST: {
@@ -2082,7 +2092,9 @@ hyle_hip_status hyle_hip_plan_launch(const hyle_hip_plan *plan, const void *cons
       b.out = outputs[0];
       b.logs = output_count > 1 ? static_cast<float *>(outputs[1]) : nullptr;
       const bool vectors = aligned(inputs[0], 16) && aligned(inputs[1], 16) && aligned(b.value, 16) && aligned(b.out, 16);
-      if (attention_tiles_serves(plan->elem, plan->attention, vectors)) err = launch_attention_tiles(plan->elem, plan->attention, b, stream);
+      if (plan->attention_few_rows && attention_split_serves(plan->elem, plan->attention, vectors))
+        err = launch_attention_split(plan->elem, plan->attention, b, plan->attention_split, workspace, stream);
+      else if (attention_tiles_serves(plan->elem, plan->attention, vectors)) err = launch_attention_tiles(plan->elem, plan->attention, b, stream);
       else err = launch_attention_general(plan->elem, plan->attention, b, stream);
       break;
     }
