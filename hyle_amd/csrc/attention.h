@@ -22,20 +22,25 @@ struct AttentionSequence {
 };
 
 // Marks are clamped to what the operands hold, so no value of theirs leads outside.
-__device__ __forceinline__ AttentionSequence attention_sequence(const AttentionParams &p, const int32_t *marks, int index) {
+__device__ __forceinline__ int attention_mark(const AttentionParams &p, const int32_t *marks, int index) {
+  return marks != nullptr ? max(marks[index], 0) : p.keys;
+}
+// A sequence of a batch or a paged cache, by its mark.
+__device__ __forceinline__ AttentionSequence attention_sequence_of(const AttentionParams &p, int index, int mark) {
   AttentionSequence s;
-  if (p.kind == AttentionKind::kPacked) {
-    const int begin = min(max(marks[index], 0), p.rows), end = min(max(marks[index + 1], begin), p.rows);
-    s.rows = s.keys = end - begin;
-    s.first = 0;
-    s.row = begin;
-  } else {
-    const int length = marks != nullptr ? max(marks[index], 0) : p.keys;
-    s.rows = p.rows;
-    s.keys = min(length, p.keys);
-    s.first = (p.kind == AttentionKind::kPaged ? length : p.keys) - p.rows;
-    s.row = (int64_t)index * p.rows;
-  }
+  s.rows = p.rows;
+  s.keys = min(mark, p.keys);
+  s.first = (p.kind == AttentionKind::kPaged ? mark : p.keys) - p.rows;
+  s.row = (int64_t)index * p.rows;
+  return s;
+}
+__device__ __forceinline__ AttentionSequence attention_sequence(const AttentionParams &p, const int32_t *marks, int index) {
+  if (p.kind != AttentionKind::kPacked) return attention_sequence_of(p, index, attention_mark(p, marks, index));
+  AttentionSequence s;
+  const int begin = min(max(marks[index], 0), p.rows), end = min(max(marks[index + 1], begin), p.rows);
+  s.rows = s.keys = end - begin;
+  s.first = 0;
+  s.row = begin;
   return s;
 }
 

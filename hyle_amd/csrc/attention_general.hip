@@ -37,7 +37,7 @@ __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_rows(AttentionP
   const AttentionSequence s = attention_sequence(p, b.marks, index);
   const AttentionSpan span = attention_span(p, s.keys, s.first + row);
   const unsigned char *q = attention_query(p, b, s, index, row, head);
-  const int group = head / p.shared, wave = (int)threadIdx.x / kWaveLanes, lane = (int)threadIdx.x % kWaveLanes;
+  const int group = (int)p.shared.quotient((uint32_t)head), wave = (int)threadIdx.x / kWaveLanes, lane = (int)threadIdx.x % kWaveLanes;
   for (int d = threadIdx.x; d < p.depth; d += kWaves * kWaveLanes) query[d] = Traits<T>::load(q, d) * p.scale;
   __syncthreads();
 

@@ -32,10 +32,10 @@ __device__ __forceinline__ SplitTiles tiles_of(const AttentionParams &p, const A
   return t;
 }
 
-// The sequence and chunk of a slot.  Every wave of a launch comes to the same answer from the marks alone.
 struct SplitChunk {
   int index, chunk, chunks;  // sequence, which of its chunks, how many it has
   int first_slot, tiles_each;
+  int mark;  // the sequence's
 };
 __device__ __forceinline__ uint32_t scanned(uint32_t v, int lane) {
   uint32_t up;
@@ -47,23 +47,30 @@ __device__ __forceinline__ uint32_t scanned(uint32_t v, int lane) {
   up = lane_up<32>(v), v += lane >= 32 ? up : 0u;
   return v;
 }
-__device__ __forceinline__ int tiles_each(const AttentionParams &p, const int32_t *marks, int target) {
+// The sequence and chunk that a slot of the grid is; false past the last.  Every wave of a launch comes to the same answer
+// from the marks alone.  target, chunks that all tiles are dealt to, is 0 where every sequence is one.  A block of one tile has
+// nothing to load while it computes, so a chunk has two at least where the tiles are more than the resident blocks.
+__device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t *marks, int slot, int target, int blocks, SplitChunk *c) {
   const int lane = (int)threadIdx.x % kWaveLanes;
-  uint64_t total = 0;
-  for (int base = 0; base < p.sequences; base += kWaveLanes) {
-    uint32_t mine = 0;
-    if (base + lane < p.sequences) mine = (uint32_t)tiles_of(p, attention_sequence(p, marks, base + lane)).tiles;
-    total += (uint32_t)__builtin_amdgcn_readlane((int)scanned(mine, lane), kWaveLanes - 1);  // (64 sequences of 2^24 tiles at most)
+  if (target == 0) {
+    if (slot >= p.sequences) return false;
+    *c = SplitChunk{slot, 0, 1, slot, 1 << 24, __builtin_amdgcn_readfirstlane(attention_mark(p, marks, slot))};
+    return true;
   }
-  const uint64_t each = (total + (uint32_t)target - 1) / (uint32_t)target;
-  return (int)(each < 1 ? 1 : each);
-}
-__device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t *marks, int slot, int each, SplitChunk *c) {
-  const int lane = (int)threadIdx.x % kWaveLanes;
+  auto tiles_at = [&](int index, int mark) { return index < p.sequences ? (uint32_t)tiles_of(p, attention_sequence_of(p, index, mark)).tiles : 0u; };
+  const int first_mark = attention_mark(p, marks, min(lane, p.sequences - 1));
+  const uint32_t first = tiles_at(lane, first_mark);  // (64 sequences of 2^24 tiles at most fit 32 bits)
+  uint64_t total = (uint32_t)__builtin_amdgcn_readlane((int)scanned(first, lane), kWaveLanes - 1);
+  for (int base = kWaveLanes; base < p.sequences; base += kWaveLanes) {
+    const int index = base + lane;
+    total += (uint32_t)__builtin_amdgcn_readlane((int)scanned(tiles_at(index, attention_mark(p, marks, min(index, p.sequences - 1))), lane), kWaveLanes - 1);
+  }
+  const int each = (int)max((total + (uint32_t)target - 1) / (uint32_t)target, total > (uint32_t)blocks ? 2ull : 1ull);
   int before = 0;
   for (int base = 0; base < p.sequences; base += kWaveLanes) {
-    uint32_t mine = 0;
-    if (base + lane < p.sequences) mine = (uint32_t)max(1, (tiles_of(p, attention_sequence(p, marks, base + lane)).tiles + each - 1) / each);
+    const int index = base + lane, mark = base == 0 ? first_mark : attention_mark(p, marks, min(index, p.sequences - 1));
+    const uint32_t tiles = base == 0 ? first : tiles_at(index, mark);
+    const uint32_t mine = index < p.sequences ? max(1u, (tiles + (uint32_t)each - 1) / (uint32_t)each) : 0u;
     const uint32_t through = scanned(mine, lane);
     const uint64_t holds = __ballot(slot < before + (int)through);
     if (holds != 0) {
@@ -73,6 +80,7 @@ __device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t
       c->first_slot = before + __builtin_amdgcn_readlane((int)through, at) - c->chunks;
       c->chunk = slot - c->first_slot;
       c->tiles_each = each;
+      c->mark = __builtin_amdgcn_readlane(mark, at);
       return true;
     }
     before += __builtin_amdgcn_readlane((int)through, kWaveLanes - 1);
@@ -117,61 +125,52 @@ __device__ __forceinline__ float rows_sum(float v) {
 }
 
 struct SplitLayout {
-  int target;     // chunks that all tiles are dealt to
+  int target;     // chunks that all tiles are dealt to, 0: none is split
+  int blocks;     // resident at once, of one key head and tile of rows
   int rows;       // query rows of a key head: query heads of it x new tokens, token by token
-  int row_tiles;  // of 16 kBlocks
+  Divisor row_tiles, lanes, lines;  // tiles of 16 kBlocks rows; those of all key heads; rows of all key heads
   float *partial; // [slots, heads, rows, depth]
   float2 *stats;  // [slots, heads, rows]: m, l
+  int2 *places;   // [sequences]: first slot, chunks
 };
 
-// T: queries and outputs, C: keys and values, kDepth: padded depth, kBlocks: blocks of 16 rows
-template <class T, class C, int kDepth, int kBlocks>
-__global__ __launch_bounds__(kThreads) void attention_split(AttentionParams p, AttentionBuffers b, SplitLayout layout) {
+// T: queries and outputs, C: keys and values, kDepth: padded depth (kWhole: the depth itself), kBlocks: blocks of 16 rows
+// Blocks of a compute unit: what the registers hold of keys, values, queries and outputs without spilling.
+constexpr int resident(bool narrow, int depth, int blocks) {
+  const int size = depth * blocks;
+  if (narrow) return size <= 64 ? 4 : size <= 128 ? 3 : size <= 256 ? 2 : 1;
+  return size <= 64 ? 4 : size <= 128 || depth == 64 ? 2 : 1;
+}
+template <class T, class C, int kDepth, int kBlocks, bool kWhole>
+__global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kDepth, kBlocks)) void attention_split(AttentionParams p, AttentionBuffers b, SplitLayout layout) {
   constexpr bool kNarrow = std::is_same<C, E4M3>::value;
   constexpr int kSteps = kDepth / 32, kDims = kDepth / 16;
   constexpr int kLoad = kNarrow ? 16 : 8;                // elements of a 16-byte vector
-  constexpr int kKeyLoads = kDepth / (4 * kLoad);        // of a lane and 16 keys
-  constexpr int kValueLoads = kDepth / (2 * kLoad);      // of a lane and 32 keys
-  constexpr int kValueRow = kDepth * 2 + 32;             // 8 rows of 32 bytes fill the banks
+  constexpr int kVectors = kDepth / kLoad;               // of a row
+  constexpr int kLoads = kStep * kVectors / kWaveLanes;  // of a lane, for a step's keys or values
+  constexpr int kRow = kDepth * 2 + 32;                  // bytes of a row in LDS: 8 rows of 32 bytes fill the banks
   constexpr int kJoinRow = kDepth + 4;                   // floats
-  constexpr int kHeld = kWaves * kStep * kValueRow, kJoined = kWaves * 16 * kJoinRow * 4;
+  constexpr int kHeld = kWaves * kStep * kRow, kJoined = kWaves * 16 * kJoinRow * 4;
   __shared__ __attribute__((aligned(16))) unsigned char held[kHeld > kJoined ? kHeld : kJoined];
   __shared__ float joined_top[kWaves][16], joined_sum[kWaves][16];
 
-  const int lanes = p.heads * layout.row_tiles, slot = (int)(blockIdx.x / (uint32_t)lanes), rest = (int)(blockIdx.x % (uint32_t)lanes);
-  const int group = rest / layout.row_tiles, row_tile = rest % layout.row_tiles;
+  const int slot = (int)layout.lanes.quotient(blockIdx.x), rest = (int)blockIdx.x - slot * (int)layout.lanes.divisor;
+  const int group = (int)layout.row_tiles.quotient((uint32_t)rest), row_tile = rest - group * (int)layout.row_tiles.divisor;
   SplitChunk chunk;
-  const int each = tiles_each(p, b.marks, layout.target);
-  if (!chunk_of(p, b.marks, slot, each, &chunk)) return;
-  const AttentionSequence s = attention_sequence(p, b.marks, chunk.index);
+  if (!chunk_of(p, b.marks, slot, layout.target, layout.blocks, &chunk)) return;
+  if (layout.target != 0 && chunk.chunk == 0 && rest == 0 && threadIdx.x == 0) layout.places[chunk.index] = int2{chunk.first_slot, chunk.chunks};
+  const AttentionSequence s = attention_sequence_of(p, chunk.index, chunk.mark);
   const SplitTiles tiles = tiles_of(p, s);
-  const int begin = chunk.chunk * each, end = min(begin + each, tiles.tiles);
+  const int begin = chunk.chunk * chunk.tiles_each, end = min(begin + chunk.tiles_each, tiles.tiles);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWaveLanes), lane = (int)threadIdx.x % kWaveLanes;
   const int column = lane % 16, quarter = lane / 16;
   const int first_row = row_tile * 16 * kBlocks;
   // what some row of the sequence sees, and what this tile of rows does (its first and last tokens)
   const AttentionSpan any{attention_span(p, s.keys, s.first).low, attention_span(p, s.keys, s.first + s.rows - 1).high};
-  const AttentionSpan tile_first = attention_span(p, s.keys, s.first + first_row / p.shared);
-  const AttentionSpan tile_last = attention_span(p, s.keys, s.first + (min(first_row + 16 * kBlocks, layout.rows) - 1) / p.shared);
+  const AttentionSpan tile_first = attention_span(p, s.keys, s.first + (int)p.shared.quotient((uint32_t)first_row));
+  const AttentionSpan tile_last = attention_span(p, s.keys, s.first + (int)p.shared.quotient((uint32_t)min(first_row + 16 * kBlocks, layout.rows) - 1u));
 
-  // queries: a lane's row is its column, its dims those that its key loads bring: vector j holds elements
-  // (4 j + quarter) kLoad on, of which e4m3 makes two operands
-  u32x4 query[kBlocks][kSteps];
-  AttentionSpan span[kBlocks];
-  const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
-  for (int n = 0; n < kBlocks; ++n) {
-    const int row = first_row + 16 * n + column, token = min(row, layout.rows - 1) / p.shared;
-    const unsigned char *from = attention_query(p, b, s, chunk.index, token, group * p.shared + min(row, layout.rows - 1) % p.shared);
-    span[n] = attention_span(p, s.keys, s.first + token);
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      const int dim = kNarrow ? (k / 2 * 4 + quarter) * 16 + k % 2 * 8 : (4 * k + quarter) * 8;
-      u32x4 w = {0, 0, 0, 0};
-      if (row < layout.rows && dim < p.depth && p.scale != 0.0f) w = load16(from, dim / 8);
-      query[n][k] = w ^ flip;
-    }
-  }
+  // a positive c, so that the maximum of S c is that of S and hidden scores stay -inf: its sign, or a scale of 0, goes into the queries
   const float c = p.scale == 0.0f ? 1.0f : fabsf(p.scale) * kLog2E;
 
   f32x4 out[kBlocks][kDims];
@@ -188,89 +187,110 @@ __global__ __launch_bounds__(kThreads) void attention_split(AttentionParams p, A
   const bool paged = p.kind == AttentionKind::kPaged;
   const int32_t *table = paged ? b.table + (int64_t)chunk.index * p.table_row : nullptr;
   auto first_key = [&](int tile) { return (tile < tiles.sinks ? tile * kTile : tiles.low + (tile - tiles.sinks) * kTile) + wave * kStep; };
-  // a lane's two keys of a step: its column and 16 on; past the last key the last one's place is asked for
-  auto pages = [&](int tile, int (&page)[2]) {
+  // A lane's key of a step, and the page that holds it; past the last key the last one's place is asked for.
+  auto page_of = [&](int tile) {
+    return paged ? table[p.page.quotient((uint32_t)min(first_key(tile) + lane % kStep, any.high - 1))] : 0;
+  };
+  // One step's keys and values, whole rows side by side: a load's 64 vectors are whole cache lines, which non-temporal loads
+  // need.  The next keys are asked for once these are in LDS, and so are the values.
+  u32x4 key_words[kLoads], value_words[kLoads];
+  uint32_t alive = 0;  // bit j: key j of the step is there and some row sees it
+  int64_t value_at = 0;
+  const int vectors = p.depth / kLoad;  // of a row; zeros past them
+  const int vector = lane % kVectors;
+  auto fetch = [&](const unsigned char *from, int64_t place, u32x4 (&words)[kLoads]) {
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      page[sub] = 0;
-      if (paged) page[sub] = table[p.page.quotient((uint32_t)min(first_key(tile) + 16 * sub + column, any.high - 1))];
+    for (int k = 0; k < kLoads; ++k) {
+      const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
+      const int64_t at = ((int64_t)__shfl((int)(place >> 32), row, kWaveLanes) << 32) | (uint32_t)__shfl((int)place, row, kWaveLanes);
+      if (!kWhole) words[k] = u32x4{0, 0, 0, 0};
+      if (kWhole || vector < vectors) words[k] = load16_stream(from + at, vector);
     }
   };
-  u32x4 next_keys[2][kKeyLoads], next_values[kValueLoads];
-  uint32_t next_alive;  // bit j: key j of the step is there and some row sees it
-  auto fetch = [&](int tile, const int (&page)[2]) {
-    int64_t key_at[2], value_at[2];
-    bool there[2];
+  auto fetch_keys = [&](int tile, int page) {
+    const int key = first_key(tile) + lane % kStep, known = min(key, any.high - 1);
+    bool there = attention_sees(p, any, key);
+    int64_t key_at;
+    if (paged) {
+      there = there && (uint32_t)page < (uint32_t)p.pages;
+      const uint32_t at = (uint32_t)known - p.page.quotient((uint32_t)known) * p.page.divisor;
+      // (a page that is not there is read as the cache's first row, which is there: its keys are not alive)
+      key_at = value_at = there ? (int64_t)page * p.k_sequence + (int64_t)at * p.k_row : 0;
+    } else {
+      key_at = (int64_t)chunk.index * p.k_sequence + (int64_t)known * p.k_row;
+      value_at = (int64_t)chunk.index * p.v_sequence + (int64_t)known * p.v_row;
+    }
+    alive = (uint32_t)__ballot(there);
+    fetch(keys, key_at, key_words);
+  };
+  // a step's vectors to the wave's rows in LDS, e4m3 as the elements of T that they stand for
+  auto put = [&](const u32x4 (&words)[kLoads]) {
+    __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses are in order)
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      const int key = first_key(tile) + 16 * sub + column, known = min(key, any.high - 1);
-      there[sub] = attention_sees(p, any, key);
-      if (paged) {
-        there[sub] = there[sub] && (uint32_t)page[sub] < (uint32_t)p.pages;
-        const uint32_t at = (uint32_t)known - p.page.quotient((uint32_t)known) * p.page.divisor;
-        // (a page that is not there is read as the cache's first row, which is there: its keys are not alive)
-        key_at[sub] = value_at[sub] = there[sub] ? (int64_t)page[sub] * p.k_sequence + (int64_t)at * p.k_row : 0;
+    for (int k = 0; k < kLoads; ++k) {
+      const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
+      unsigned char *to = held + (wave * kStep + row) * kRow + vector * kLoad * 2;
+      if constexpr (kNarrow) {
+        u32x4 low, high;
+        widened<T>(words[k], &low, &high);
+        *reinterpret_cast<u32x4 *>(to) = low;
+        *reinterpret_cast<u32x4 *>(to + 16) = high;
       } else {
-        key_at[sub] = (int64_t)chunk.index * p.k_sequence + (int64_t)known * p.k_row;
-        value_at[sub] = (int64_t)chunk.index * p.v_sequence + (int64_t)known * p.v_row;
+        *reinterpret_cast<u32x4 *>(to) = words[k];
       }
     }
-    next_alive = ((uint32_t)__ballot(there[0]) & 0xFFFFu) | ((uint32_t)__ballot(there[1]) << 16);
-    const int last = p.depth / kLoad - 1;  // vectors past the depth: the row's last one, in whose place zeros are used
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-      for (int k = 0; k < kKeyLoads; ++k) next_keys[sub][k] = load16(keys + key_at[sub], (size_t)min(4 * k + quarter, last));
-    const int64_t at = (lane & 16) != 0 ? value_at[1] : value_at[0];
-#pragma unroll
-    for (int k = 0; k < kValueLoads; ++k) next_values[k] = load16(values + at, (size_t)min(2 * k + lane / 32, last));
+    __builtin_amdgcn_wave_barrier();  // other lanes' rows are read next
   };
 
-  unsigned char *rows = held + wave * kStep * kValueRow;
-  int page[2], next_page[2] = {0, 0};
+  unsigned char *rows = held + wave * kStep * kRow;
+  int page = 0;
+  if (begin < end) page = page_of(begin);
+  // queries: a lane's row is its column, its dims 8 quarter on of every 32
+  u32x4 query[kBlocks][kSteps];
+  AttentionSpan span[kBlocks];
+#pragma unroll
+  for (int n = 0; n < kBlocks; ++n) {
+    const int row = first_row + 16 * n + column, known = min(row, layout.rows - 1), token = (int)p.shared.quotient((uint32_t)known);
+    const unsigned char *from = attention_query(p, b, s, chunk.index, token, group * (int)p.shared.divisor + known - token * (int)p.shared.divisor);
+    span[n] = attention_span(p, s.keys, s.first + token);
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      query[n][k] = u32x4{0, 0, 0, 0};
+      if (row < layout.rows && (kWhole || (4 * k + quarter) * 8 < p.depth)) query[n][k] = load16(from, 4 * k + quarter);
+    }
+  }
   if (begin < end) {
-    pages(begin, page);
-    if (begin + 1 < end) pages(begin + 1, next_page);
-    fetch(begin, page);
+    fetch_keys(begin, page);
+    fetch(values, value_at, value_words);
+    if (begin + 1 < end) page = page_of(begin + 1);
+  }
+  if (p.scale <= 0.0f) {
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) query[n][k] = p.scale == 0.0f ? u32x4{0, 0, 0, 0} : query[n][k] ^ 0x80008000u;
   }
   for (int tile = begin; tile < end; ++tile) {
-    u32x4 key_words[2][kKeyLoads], value_words[kValueLoads];
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-      for (int k = 0; k < kKeyLoads; ++k) key_words[sub][k] = next_keys[sub][k];
-#pragma unroll
-    for (int k = 0; k < kValueLoads; ++k) value_words[k] = next_values[k];
-    const uint32_t alive = next_alive;
-    if (tile + 1 < end) {
-      page[0] = next_page[0], page[1] = next_page[1];
-      if (tile + 2 < end) pages(tile + 2, next_page);
-      fetch(tile + 1, page);
-    }
-    if (alive == 0) continue;
+    const uint32_t these = alive;
     const int first = first_key(tile);
-    const bool whole = alive == 0xFFFFFFFFu && first + kStep <= tile_first.high && first >= tile_last.low;
+    const bool whole = these == 0xFFFFFFFFu && first + kStep <= tile_first.high && first >= tile_last.low;
 
+    put(key_words);
+    __builtin_amdgcn_sched_barrier(0);  // (loads that move up further need registers of their own)
+    if (tile + 1 < end) {
+      fetch_keys(tile + 1, page);
+      if (tile + 2 < end) page = page_of(tile + 2);
+    }
     f32x4 score[kBlocks][2];
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
 #pragma unroll
       for (int n = 0; n < kBlocks; ++n) score[n][sub] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int k = 0; k < kKeyLoads; ++k) {
-        u32x4 w = key_words[sub][k];
-        if (p.depth != kDepth && (4 * k + quarter) * kLoad >= p.depth) w = u32x4{0, 0, 0, 0};
-        if constexpr (kNarrow) {
-          u32x4 low, high;
-          widened<T>(w, &low, &high);
+      for (int k = 0; k < kSteps; ++k) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(rows + (16 * sub + column) * kRow + (4 * k + quarter) * 16);
 #pragma unroll
-          for (int n = 0; n < kBlocks; ++n) score[n][sub] = product16<T>(low, query[n][2 * k], score[n][sub]);
-#pragma unroll
-          for (int n = 0; n < kBlocks; ++n) score[n][sub] = product16<T>(high, query[n][2 * k + 1], score[n][sub]);
-        } else {
-#pragma unroll
-          for (int n = 0; n < kBlocks; ++n) score[n][sub] = product16<T>(w, query[n][k], score[n][sub]);
-        }
+        for (int n = 0; n < kBlocks; ++n) score[n][sub] = product16<T>(w, query[n][k], score[n][sub]);
       }
     }
     if (!whole) {
@@ -281,7 +301,7 @@ __global__ __launch_bounds__(kThreads) void attention_split(AttentionParams p, A
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int j = 16 * sub + 4 * quarter + r;
-            if (((alive >> j) & 1u) == 0 || !attention_sees(p, span[n], first + j)) score[n][sub][r] = -INFINITY;
+            if (((these >> j) & 1u) == 0 || !attention_sees(p, span[n], first + j)) score[n][sub][r] = -INFINITY;
           }
     }
     float most[kBlocks];
@@ -320,65 +340,53 @@ __global__ __launch_bounds__(kThreads) void attention_split(AttentionParams p, A
       }
     }
 
-    // values to the wave's rows in LDS; keys that are not alive bring zeros
-    const bool mine = ((alive >> (lane % 32)) & 1u) != 0;
-    auto put = [&]() {
+    // keys that are not alive bring zeros
+    if (these != 0xFFFFFFFFu) {
 #pragma unroll
-      for (int k = 0; k < kValueLoads; ++k) {
-        unsigned char *to = rows + lane % 32 * kValueRow + (2 * k + lane / 32) * kLoad * 2;
-        const u32x4 w = value_words[k];
-        if constexpr (kNarrow) {
-          u32x4 low, high;
-          widened<T>(w, &low, &high);
-          *reinterpret_cast<u32x4 *>(to) = low;
-          *reinterpret_cast<u32x4 *>(to + 16) = high;
-        } else {
-          *reinterpret_cast<u32x4 *>(to) = w;
-        }
+      for (int k = 0; k < kLoads; ++k) {
+        const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
+        if (((these >> row) & 1u) == 0) value_words[k] = u32x4{0, 0, 0, 0};
       }
-      __builtin_amdgcn_wave_barrier();  // other lanes' rows are read next: a wave's LDS accesses are in order
-    };
-    if (alive != 0xFFFFFFFFu) {
-#pragma unroll
-      for (int k = 0; k < kValueLoads; ++k) value_words[k] = mine ? value_words[k] : u32x4{0, 0, 0, 0};
     }
     if (!whole && s.rows > 1) {
       // Values that are no numbers, of keys that not every row sees: a weight of 0 would make NaN of them in the product.
       // They are added to the rows that see them (a finite weight changes nothing about them) and zeroed.
       uint32_t found = 0;
 #pragma unroll
-      for (int k = 0; k < kValueLoads; ++k) found |= no_numbers<C>(value_words[k]);
+      for (int k = 0; k < kLoads; ++k) found |= no_numbers<C>(value_words[k]);
       if (__ballot(found != 0) != 0) {
-        put();
+        put(value_words);
         for (int j = 0; j < kStep; ++j) {
-          if (((alive >> j) & 1u) == 0) continue;
+          if (((these >> j) & 1u) == 0) continue;
 #pragma unroll
-          for (int n = 0; n < kBlocks; ++n) {
-            const bool sees = attention_sees(p, span[n], first + j);
+          for (int d = 0; d < kDims; ++d) {
+            float v[4];
 #pragma unroll
-            for (int d = 0; d < kDims; ++d)
+            for (int r = 0; r < 4; ++r) {
+              const float x = Traits<T>::load(rows + j * kRow, 16 * d + 4 * quarter + r);
+              v[r] = fabsf(x) < INFINITY ? 0.0f : x;
+            }
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float v = Traits<T>::load(rows + j * kValueRow, 16 * d + 4 * quarter + r);
-                if (sees && !(fabsf(v) < INFINITY)) out[n][d][r] += v;
-              }
+            for (int n = 0; n < kBlocks; ++n)
+              if (attention_sees(p, span[n], first + j)) out[n][d] += f32x4{v[0], v[1], v[2], v[3]};
+            asm volatile("" : : : "memory");  // (a dim at a time: all at once would cost every step its registers)
           }
         }
-        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int k = 0; k < kValueLoads; ++k) value_words[k] = numbers_only<C>(value_words[k]);
+        for (int k = 0; k < kLoads; ++k) value_words[k] = numbers_only<C>(value_words[k]);
       }
     }
-    put();
+    put(value_words);
+    __builtin_amdgcn_sched_barrier(0);
+    if (tile + 1 < end) fetch(values, value_at, value_words);
 #pragma unroll
     for (int d = 0; d < kDims; ++d) {
-      const unsigned char *at = rows + (4 * quarter + column / 4) * kValueRow + (d * 16 + column % 4 * 4) * 2;
-      const uint2 near = read_transposed(at), far = read_transposed(at + 16 * kValueRow);
+      const unsigned char *at = rows + (4 * quarter + column / 4) * kRow + (d * 16 + column % 4 * 4) * 2;
+      const uint2 near = read_transposed(at), far = read_transposed(at + 16 * kRow);
       const u32x4 value = {near.x, near.y, far.x, far.y};
 #pragma unroll
       for (int n = 0; n < kBlocks; ++n) out[n][d] = product16<T>(value, weights[n], out[n][d]);
     }
-    __builtin_amdgcn_wave_barrier();
   }
 
   // join the waves, 16 rows at a time
@@ -404,7 +412,8 @@ __global__ __launch_bounds__(kThreads) void attention_split(AttentionParams p, A
         keep[w] = __builtin_amdgcn_exp2f(joined_top[w][join_row] - shift);
         all += joined_sum[w][join_row] * keep[w];
       }
-      const int64_t at = (s.row + row / p.shared) * p.queries + group * p.shared + row % p.shared;
+      const int token = (int)p.shared.quotient((uint32_t)row);
+      const int64_t at = (s.row + token) * p.queries + group * (int)p.shared.divisor + row - token * (int)p.shared.divisor;
       const int64_t part = ((int64_t)slot * p.heads + group) * layout.rows + row;
       const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
       for (int d = (int)threadIdx.x % 16 * 4; d < p.depth; d += 64) {
@@ -422,70 +431,64 @@ __global__ __launch_bounds__(kThreads) void attention_split(AttentionParams p, A
       }
       if (threadIdx.x % 16 == 0) {
         if (chunk.chunks != 1) layout.stats[part] = float2{most, all};
-        else if (b.logs != nullptr) b.logs[at] = all == 0.0f ? -INFINITY : most * kLn2 + logf(all);
+        else if (b.logs != nullptr) b.logs[at] = all == 0.0f ? -INFINITY : (most + __builtin_amdgcn_logf(all)) * kLn2;
       }
     }
   }
 }
 
-// The chunks of one query row joined: kThreads / kDepth chunks side by side, a dim to a thread.
+constexpr int join_threads(int depth) { return depth == 256 ? 512 : 256; }
+// The chunks of one query row joined: four dims to a thread, kParts chunks side by side.
 template <class T, int kDepth>
-__global__ __launch_bounds__(kThreads) void attention_join(AttentionParams p, AttentionBuffers b, SplitLayout layout) {
-  constexpr int kParts = kThreads / kDepth;
-  __shared__ float joined[kParts][kDepth], tops[kParts], sums[kParts];
-  const int lines = p.heads * layout.rows, index = (int)(blockIdx.x / (uint32_t)lines), rest = (int)(blockIdx.x % (uint32_t)lines);
-  const int group = rest / layout.rows, row = rest % layout.rows;
-  const int each = tiles_each(p, b.marks, layout.target);
-  // the slots before this sequence's
-  int before = 0, chunks = 0;
+__global__ __launch_bounds__(join_threads(kDepth)) void attention_join(AttentionParams p, AttentionBuffers b, SplitLayout layout) {
+  constexpr int kLanes = kDepth / 4, kParts = join_threads(kDepth) / kLanes;
+  __shared__ __attribute__((aligned(16))) f32x4 joined[kParts][kLanes];
+  __shared__ float sums[kParts];
+  const int index = (int)layout.lines.quotient(blockIdx.x), rest = (int)blockIdx.x - index * (int)layout.lines.divisor;  // key head and row
+  const int2 place = layout.places[index];
+  if (place.y == 1) return;  // the split kernel's block was the whole sequence
+  const int64_t stride = (int64_t)p.heads * layout.rows, first = (int64_t)place.x * stride + rest;
   const int lane = (int)threadIdx.x % kWaveLanes;
-  for (int base = 0; base <= index; base += kWaveLanes) {
-    uint32_t mine = 0;
-    if (base + lane <= index) mine = (uint32_t)max(1, (tiles_of(p, attention_sequence(p, b.marks, base + lane)).tiles + each - 1) / each);
-    before += __builtin_amdgcn_readlane((int)scanned(mine, lane), kWaveLanes - 1);
-    chunks = __builtin_amdgcn_readlane((int)mine, index % kWaveLanes);  // (of the last round)
-  }
-  if (chunks == 1) return;  // the split kernel's block was the whole sequence
-  before -= chunks;
-  const AttentionSequence s = attention_sequence(p, b.marks, index);
-  const int dim = (int)threadIdx.x % kDepth, part = (int)threadIdx.x / kDepth;
-  const int64_t first = ((int64_t)before * p.heads + group) * layout.rows + row, stride = (int64_t)p.heads * layout.rows;
-  float most = -INFINITY;
-  for (int i = part; i < chunks; i += kParts) most = fmaxf(most, layout.stats[first + i * stride].x);
+  float most = -INFINITY;  // every wave looks at all chunks' maxima
+  for (int i = lane; i < place.y; i += kWaveLanes) most = fmaxf(most, layout.stats[first + i * stride].x);
+  most = group_max<kWaveLanes>(most);
   const float shift = most == -INFINITY ? 0.0f : most;
-  float out = 0.0f, sum = 0.0f;
-#pragma unroll 4
-  for (int i = part; i < chunks; i += kParts) {
+  const int dim = (int)threadIdx.x % kLanes * 4, part = (int)threadIdx.x / kLanes;
+  f32x4 out = {0.0f, 0.0f, 0.0f, 0.0f};
+  float sum = 0.0f;
+  const bool has = dim < p.depth;
+#pragma unroll 8
+  for (int i = part; i < place.y; i += kParts) {
     const float2 stat = layout.stats[first + i * stride];
+    const f32x4 o = *reinterpret_cast<const f32x4 *>(layout.partial + (first + i * stride) * p.depth + (has ? dim : 0));
     const float keep = __builtin_amdgcn_exp2f(stat.x - shift);
-    sum += stat.y * keep;
-    if (dim < p.depth) out += layout.partial[(first + i * stride) * p.depth + dim] * keep;
+    sum = __builtin_fmaf(stat.y, keep, sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = __builtin_fmaf(o[e], keep, out[e]);
   }
-  joined[part][dim] = out;
-  if (dim == 0) tops[part] = most, sums[part] = sum;
+  joined[part][dim / 4] = out;
+  if (dim == 0) sums[part] = sum;
   __syncthreads();
   if (part != 0) return;
-  float all = tops[0];
 #pragma unroll
-  for (int i = 1; i < kParts; ++i) all = fmaxf(all, tops[i]);
-  const float base = all == -INFINITY ? 0.0f : all;
-  out = 0.0f, sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kParts; ++i) {
-    const float keep = __builtin_amdgcn_exp2f(tops[i] - base);
-    out += joined[i][dim] * keep;
-    sum += sums[i] * keep;
+  for (int i = 1; i < kParts; ++i) out += joined[i][dim / 4], sum += sums[i];
+  const int group = rest / layout.rows, row = rest - group * layout.rows, token = (int)p.shared.quotient((uint32_t)row);
+  const int64_t at = ((int64_t)index * p.rows + token) * p.queries + group * (int)p.shared.divisor + row - token * (int)p.shared.divisor;
+  if (has) {
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint2 w;
+    w.x = pack2<T>(out[0] * inverse, out[1] * inverse);
+    w.y = pack2<T>(out[2] * inverse, out[3] * inverse);
+    *reinterpret_cast<uint2 *>(static_cast<unsigned char *>(b.out) + (at * p.depth + dim) * 2) = w;
   }
-  const int64_t at = (s.row + row / p.shared) * p.queries + group * p.shared + row % p.shared;
-  if (dim < p.depth) Traits<T>::store(b.out, (size_t)(at * p.depth + dim), sum == 0.0f ? 0.0f : out / sum);
-  if (b.logs != nullptr && dim == 0) b.logs[at] = sum == 0.0f ? -INFINITY : all * kLn2 + logf(sum);
+  if (b.logs != nullptr && dim == 0) b.logs[at] = sum == 0.0f ? -INFINITY : (most + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 }  // namespace
 
-template <class C, int kDepth, int kBlocks> struct AttentionSplitTag {
+template <class C, int kDepth, int kBlocks, bool kWhole> struct AttentionSplitTag {
   static std::string text() {
-    return std::string("attention_split/") + (std::is_same<C, E4M3>::value ? "e4m3/d" : "d") + std::to_string(kDepth) + "/" + std::to_string(16 * kBlocks) + "-rows";
+    return std::string("attention_split/") + (std::is_same<C, E4M3>::value ? "e4m3/" : "") + (kWhole ? "d" : "below-d") + std::to_string(kDepth) + "/" + std::to_string(16 * kBlocks) + "-rows";
   }
 };
 template <int kDepth> struct AttentionJoinTag {
@@ -495,30 +498,42 @@ template <int kDepth> struct AttentionJoinTag {
 namespace {
 int padded_depth(const AttentionParams &p) { return p.depth <= 64 ? 64 : p.depth <= 128 ? 128 : 256; }
 int blocks_of(const AttentionParams &p) {
-  const int64_t rows = (int64_t)p.rows * p.shared;
+  const int64_t rows = (int64_t)p.rows * p.shared.divisor;
   return rows <= 16 ? 1 : rows <= 32 || p.depth > 128 ? 2 : 4;
 }
 int row_tiles_of(const AttentionParams &p) {
   const int64_t each = 16 * blocks_of(p);
-  return (int)(((int64_t)p.rows * p.shared + each - 1) / each);
+  return (int)(((int64_t)p.rows * p.shared.divisor + each - 1) / each);
 }
 }  // namespace
 
 AttentionSplit attention_split_of(const AttentionParams &p, int compute_units) {
   AttentionSplit split;
-  // the chunks of one key head and tile of rows: four blocks to a compute unit over all of them
+  // The chunks of one key head and tile of rows: three rounds of the blocks that the device holds, so that the last ones of
+  // ragged sequences leave it idle for a third of a block.
   const int64_t lanes = (int64_t)p.heads * row_tiles_of(p);
-  const int64_t target = ((int64_t)compute_units * 4 + lanes - 1) / lanes;
-  const int64_t most = ((int64_t)p.keys + kTile - 1) / kTile + 1;  // tiles of a sequence
+  const int64_t blocks = (int64_t)compute_units * resident(p.narrow_cache, padded_depth(p), blocks_of(p));
+  const int64_t target = (3 * blocks + lanes - 1) / lanes;
+  split.blocks = (int)((blocks + lanes - 1) / lanes);
+  // tiles of a sequence: of all its keys, or of the window of its new tokens and the sinks
+  int64_t most = ((int64_t)p.keys + kTile - 1) / kTile;
+  if (p.window != 0) {
+    const int64_t seen = ((int64_t)p.window + p.rows + kTile - 1) / kTile + 1 + ((int64_t)p.sinks + kTile - 1) / kTile;
+    if (seen < most) most = seen;
+  }
   split.target = (int)target;
-  // sum over the sequences of ceil(tiles / each) with each >= total / target
-  int64_t slots = target + p.sequences;
-  if (most * p.sequences < slots) slots = most * p.sequences;
-  split.slots = (int)(slots < p.sequences ? p.sequences : slots);
+  // The sum over the sequences of ceil(tiles / each), at least one for each of them, where each is at least total / target and,
+  // with more tiles than blocks, 2.
+  int64_t slots = most * p.sequences / 2 > split.blocks ? most * p.sequences / 2 : split.blocks;
+  if (target < slots) slots = target;
+  slots += p.sequences;
+  split.slots = (int)slots;
   split.joined = p.keys > kTile && target > 1;
-  const int64_t rows = (int64_t)p.rows * p.shared * p.heads * split.slots;
+  if (!split.joined) split.target = 0, split.slots = p.sequences;
+  const int64_t rows = (int64_t)p.rows * p.shared.divisor * p.heads * split.slots;
   split.stats_offset = ((size_t)rows * (size_t)p.depth * sizeof(float) + 255) / 256 * 256;
-  split.workspace = split.joined ? split.stats_offset + (size_t)rows * sizeof(float2) : 0;
+  split.places_offset = split.stats_offset + ((size_t)rows * sizeof(float2) + 255) / 256 * 256;
+  split.workspace = split.joined ? split.places_offset + (size_t)p.sequences * sizeof(int2) : 0;
   return split;
 }
 
@@ -530,12 +545,17 @@ bool attention_split_serves(Elem type, const AttentionParams &p, bool vector_ali
 namespace {
 template <class T, class C, int kDepth, int kBlocks>
 void start_split(const AttentionParams &p, const AttentionBuffers &b, const SplitLayout &layout, const AttentionSplit &split, hipStream_t stream) {
-  note_variant<AttentionSplitTag<C, kDepth, kBlocks>>();
-  hipLaunchKernelGGL((attention_split<T, C, kDepth, kBlocks>), dim3((uint32_t)split.slots * (uint32_t)(p.heads * layout.row_tiles)), dim3(kThreads), 0,
-                     stream, p, b, layout);
+  const dim3 grid((uint32_t)split.slots * layout.lanes.divisor), block(kThreads);
+  if (p.depth == kDepth) {
+    note_variant<AttentionSplitTag<C, kDepth, kBlocks, true>>();
+    hipLaunchKernelGGL((attention_split<T, C, kDepth, kBlocks, true>), grid, block, 0, stream, p, b, layout);
+  } else {
+    note_variant<AttentionSplitTag<C, kDepth, kBlocks, false>>();
+    hipLaunchKernelGGL((attention_split<T, C, kDepth, kBlocks, false>), grid, block, 0, stream, p, b, layout);
+  }
   if (!split.joined) return;
   note_variant<AttentionJoinTag<kDepth>>();
-  hipLaunchKernelGGL((attention_join<T, kDepth>), dim3((uint32_t)(p.heads * layout.rows) * (uint32_t)p.sequences), dim3(kThreads), 0, stream, p, b, layout);
+  hipLaunchKernelGGL((attention_join<T, kDepth>), dim3(layout.lines.divisor * (uint32_t)p.sequences), dim3(join_threads(kDepth)), 0, stream, p, b, layout);
 }
 template <class T, class C>
 void split_by_depth(const AttentionParams &p, const AttentionBuffers &b, const SplitLayout &layout, const AttentionSplit &split, hipStream_t stream) {
@@ -562,10 +582,14 @@ hipError_t launch_attention_split(Elem type, const AttentionParams &p, const Att
                                   hipStream_t stream) {
   SplitLayout layout;
   layout.target = split.target;
-  layout.rows = p.rows * p.shared;
-  layout.row_tiles = row_tiles_of(p);
+  layout.blocks = split.blocks;
+  layout.rows = p.rows * (int)p.shared.divisor;
+  layout.row_tiles = Divisor((uint32_t)row_tiles_of(p));
+  layout.lanes = Divisor((uint32_t)(p.heads * row_tiles_of(p)));
+  layout.lines = Divisor((uint32_t)(p.heads * layout.rows));
   layout.partial = static_cast<float *>(workspace);
   layout.stats = reinterpret_cast<float2 *>(static_cast<unsigned char *>(workspace) + split.stats_offset);
+  layout.places = reinterpret_cast<int2 *>(static_cast<unsigned char *>(workspace) + split.places_offset);
   if (type == Elem::kF16) {
     if (p.narrow_cache) split_by_depth<F16, E4M3>(p, b, layout, split, stream);
     else split_by_depth<F16, F16>(p, b, layout, split, stream);

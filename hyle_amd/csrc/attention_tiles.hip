@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_tiles(Attention
   int index, tile;
   if (!tile_of(p, b.marks, slot, kRows, tiles, &index, &tile)) return;
   const AttentionSequence s = attention_sequence(p, b.marks, index);
-  const int group = head / p.shared, wave = (int)threadIdx.x / kWaveLanes, lane = (int)threadIdx.x % kWaveLanes;
+  const int group = (int)p.shared.quotient((uint32_t)head), wave = (int)threadIdx.x / kWaveLanes, lane = (int)threadIdx.x % kWaveLanes;
   const int half = lane / 32, column = lane % 32;
   const int block_row = tile * kRows, wave_row = block_row + wave * 32 * kBlocks;
   const int block_last = min(block_row + kRows, s.rows) - 1, wave_last = min(wave_row + 32 * kBlocks, s.rows) - 1;
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_tiles(Attention
           *reinterpret_cast<uint2 *>(to + dim * 2) = w;
         }
       }
-    if (b.logs != nullptr && half == 0) b.logs[at] = total == 0.0f ? -INFINITY : top[q] * kLn2 + logf(total);
+    if (b.logs != nullptr && half == 0) b.logs[at] = total == 0.0f ? -INFINITY : (top[q] + __builtin_amdgcn_logf(total)) * kLn2;
   }
 }
 

@@ -385,7 +385,8 @@ struct AttentionParams {
   int32_t sequences = 0;
   int32_t rows = 0;   // of each sequence; packed: of all
   int32_t keys = 0;   // most keys of a sequence
-  int32_t queries = 0, heads = 0, shared = 1, depth = 0;  // query heads, key heads, query heads to a key head
+  int32_t queries = 0, heads = 0, depth = 0;  // query heads, key heads
+  Divisor shared;                             // query heads to a key head
   int32_t window = 0, sinks = 0;
   float scale = 1.0f;
   int64_t q_sequence = 0, q_row = 0, q_head = 0;
@@ -402,11 +403,11 @@ struct AttentionBuffers {
   void *out = nullptr;
   float *logs = nullptr;
 };
-// The split over the keys: chunks that the keys are dealt to, slots of the grid, whether a second kernel joins, the workspace.
+// The split over the keys: chunks that the keys are dealt to (0: one to a sequence), slots of the grid, whether a second kernel joins, the workspace.
 struct AttentionSplit {
-  int target = 1, slots = 0;
+  int target = 1, blocks = 1, slots = 0;
   bool joined = false;
-  size_t stats_offset = 0, workspace = 0;
+  size_t stats_offset = 0, places_offset = 0, workspace = 0;
 };
 AttentionSplit attention_split_of(const AttentionParams &p, int compute_units);
 bool attention_split_serves(Elem type, const AttentionParams &p, bool vector_aligned);

@@ -1005,12 +1005,12 @@ hyle_hip_status admit_attention(hyle_hip_plan *p, uint32_t units) {
     a.v_head = value.byte_strides[row + 1];
     if (packed && a.sequences == 0) return HYLE_HIP_OK;  // every row is behind the last sequence
   }
-  a.shared = a.queries / a.heads;
+  a.shared = Divisor((uint32_t)(a.queries / a.heads));
   for (uint32_t i = 0; i < r.input_count; ++i) p->concat_input_bytes[i] = spanned_bytes(in[i]);
   p->route = Route::kAttention;
   p->dispatches = 1;
   // few rows to a key head leave the tiles of 128 rows empty and the device too, so the keys are split instead
-  p->attention_few_rows = paged || (!packed && (int64_t)a.rows * a.shared <= 64);
+  p->attention_few_rows = paged || (!packed && (int64_t)a.rows * a.shared.divisor <= 64);
   if (p->attention_few_rows && attention_split_serves(p->elem, a, true)) {
     p->attention_split = attention_split_of(a, (int)units);
     p->workspace_size = p->attention_split.workspace;
