@@ -61,7 +61,7 @@ __device__ __forceinline__ bool tile_of(const AttentionParams &p, const int32_t 
 }
 
 template <class T, int kDepth, int kWaves, int kBlocks, int kKeys>
-__global__ __launch_bounds__(kWaves * kWaveLanes) void attention_tiles(AttentionParams p, AttentionBuffers b, int tiles) {
+__global__ __launch_bounds__(kWaves * kWaveLanes, kDepth <= 64 ? 3 : kDepth <= 128 ? 2 : 1) void attention_tiles(AttentionParams p, AttentionBuffers b, int tiles) {
   constexpr int kThreads = kWaves * kWaveLanes, kRows = kWaves * 32 * kBlocks;
   constexpr int kChunks = kDepth / 8;                       // 16-byte vectors of a row
   constexpr int kKeyRow = kDepth * 2 + 16;                  // 8 rows on in LDS lie in other banks
@@ -194,6 +194,7 @@ __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_tiles(Attention
         }
       }
       if (!(first + kKeys <= wave_first.high && first >= wave_end.low)) {
+        asm volatile("" : : : "memory");  // (a branch: as selects, the comparisons cost every step a third of its instructions)
 #pragma unroll
         for (int q = 0; q < kBlocks; ++q) {
           const AttentionSpan span = attention_span(p, s.keys, s.first + wave_row + 32 * q + column);
@@ -255,18 +256,21 @@ __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_tiles(Attention
       // Values that are no numbers, in a step that not every row sees whole: a weight of 0 would make NaN of them in the
       // product.  They are added to the rows that see them (a finite weight changes nothing about them) and zeroed.
       if (!idle) {
+#pragma unroll 1
         for (int j = 0; j < kKeys; ++j) {
 #pragma unroll
           for (int q = 0; q < kBlocks; ++q) {
             const AttentionSpan span = attention_span(p, s.keys, s.first + wave_row + 32 * q + column);
             const bool sees = attention_sees(p, span, first + j);
 #pragma unroll
-            for (int d = 0; d < kDims; ++d)
+            for (int d = 0; d < kDims; ++d) {
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
                 const float v = Traits<T>::load(value_rows + j * kValueRow, 32 * d + 8 * (r / 4) + 4 * half + r % 4);
                 if (sees && !(fabsf(v) < INFINITY)) out[q][d][r] += v;
               }
+              asm volatile("" : : : "memory");  // (a block of dims at a time: all at once would cost every step its registers)
+            }
           }
         }
       }
