@@ -128,21 +128,21 @@ struct SplitLayout {
   int target;     // chunks that all tiles are dealt to, 0: none is split
   int blocks;     // resident at once, of one key head and tile of rows
   int rows;       // query rows of a key head: query heads of it x new tokens, token by token
-  Divisor row_tiles, lanes, lines;  // tiles of 16 kBlocks rows; those of all key heads; rows of all key heads
+  Divisor row_tiles, lanes, lines;  // tiles of 16 kRowWaves rows; those of all key heads; rows of all key heads
   float *partial; // [slots, heads, rows, depth]
   float2 *stats;  // [slots, heads, rows]: m, l
   int2 *places;   // [sequences]: first slot, chunks
 };
 
-// T: queries and outputs, C: keys and values, kDepth: padded depth (kWhole: the depth itself), kBlocks: blocks of 16 rows
-// Blocks of a compute unit: what the registers hold of keys, values, queries and outputs without spilling.
-constexpr int resident(bool narrow, int depth, int blocks) {
-  const int size = depth * blocks;
-  if (narrow) return size <= 64 ? 4 : size <= 128 ? 3 : size <= 256 ? 2 : 1;
-  return size <= 64 ? 4 : size <= 128 || depth == 64 ? 2 : 1;
+// T: queries and outputs, C: keys and values, kDepth: padded depth (kWhole: the depth itself), kRowWaves: waves of 16 rows each that share a tile's
+// keys (1: every wave has all rows and its own keys)
+// Blocks of a compute unit: what the registers hold of keys, values, queries and outputs without spilling, and LDS of shared keys.
+constexpr int resident(bool narrow, int depth, int row_waves) {
+  if (row_waves > 1) return depth <= 64 ? 3 : depth <= 128 ? 2 : 1;
+  return depth <= 64 ? 4 : depth <= 128 ? (narrow ? 3 : 2) : narrow ? 2 : 1;
 }
-template <class T, class C, int kDepth, int kBlocks, bool kWhole>
-__global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kDepth, kBlocks)) void attention_split(AttentionParams p, AttentionBuffers b, SplitLayout layout) {
+template <class T, class C, int kDepth, int kRowWaves, bool kWhole>
+__global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kDepth, kRowWaves)) void attention_split(AttentionParams p, AttentionBuffers b, SplitLayout layout) {
   constexpr bool kNarrow = std::is_same<C, E4M3>::value;
   constexpr int kSteps = kDepth / 32, kDims = kDepth / 16;
   constexpr int kLoad = kNarrow ? 16 : 8;                // elements of a 16-byte vector
@@ -150,9 +150,12 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
   constexpr int kLoads = kStep * kVectors / kWaveLanes;  // of a lane, for a step's keys or values
   constexpr int kRow = kDepth * 2 + 32;                  // bytes of a row in LDS: 8 rows of 32 bytes fill the banks
   constexpr int kJoinRow = kDepth + 4;                   // floats
-  constexpr int kHeld = kWaves * kStep * kRow, kJoined = kWaves * 16 * kJoinRow * 4;
+  constexpr int kGroups = kWaves / kRowWaves;            // of waves that have keys of their own
+  constexpr int kHeld = (kRowWaves == 1 ? 1 : 2) * kWaves * kStep * kRow, kJoined = kWaves * 16 * kJoinRow * 4;
   __shared__ __attribute__((aligned(16))) unsigned char held[kHeld > kJoined ? kHeld : kJoined];
   __shared__ float joined_top[kWaves][16], joined_sum[kWaves][16];
+  __shared__ uint32_t shared_alive[kWaves];
+  __shared__ int no_number;  // 1 + the tile whose values hold an infinity or NaN
 
   const int slot = (int)layout.lanes.quotient(blockIdx.x), rest = (int)blockIdx.x - slot * (int)layout.lanes.divisor;
   const int group = (int)layout.row_tiles.quotient((uint32_t)rest), row_tile = rest - group * (int)layout.row_tiles.divisor;
@@ -164,29 +167,27 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
   const int begin = chunk.chunk * chunk.tiles_each, end = min(begin + chunk.tiles_each, tiles.tiles);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWaveLanes), lane = (int)threadIdx.x % kWaveLanes;
   const int column = lane % 16, quarter = lane / 16;
-  const int first_row = row_tile * 16 * kBlocks;
+  const int row_wave = wave % kRowWaves, key_group = wave / kRowWaves;
+  const int first_row = row_tile * 16 * kRowWaves;
   // what some row of the sequence sees, and what this tile of rows does (its first and last tokens)
   const AttentionSpan any{attention_span(p, s.keys, s.first).low, attention_span(p, s.keys, s.first + s.rows - 1).high};
   const AttentionSpan tile_first = attention_span(p, s.keys, s.first + (int)p.shared.quotient((uint32_t)first_row));
-  const AttentionSpan tile_last = attention_span(p, s.keys, s.first + (int)p.shared.quotient((uint32_t)min(first_row + 16 * kBlocks, layout.rows) - 1u));
+  const AttentionSpan tile_last = attention_span(p, s.keys, s.first + (int)p.shared.quotient((uint32_t)min(first_row + 16 * kRowWaves, layout.rows) - 1u));
 
   // a positive c, so that the maximum of S c is that of S and hidden scores stay -inf: its sign, or a scale of 0, goes into the queries
   const float c = p.scale == 0.0f ? 1.0f : fabsf(p.scale) * kLog2E;
 
-  f32x4 out[kBlocks][kDims];
-  float top[kBlocks], sum[kBlocks];
+  f32x4 out[kDims];
+  float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-  for (int n = 0; n < kBlocks; ++n) {
-    top[n] = -INFINITY, sum[n] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < kDims; ++d) out[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int d = 0; d < kDims; ++d) out[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   const unsigned char *keys = static_cast<const unsigned char *>(b.key) + (int64_t)group * p.k_head;
   const unsigned char *values = static_cast<const unsigned char *>(b.value) + (int64_t)group * p.v_head;
   const bool paged = p.kind == AttentionKind::kPaged;
   const int32_t *table = paged ? b.table + (int64_t)chunk.index * p.table_row : nullptr;
-  auto first_key = [&](int tile) { return (tile < tiles.sinks ? tile * kTile : tiles.low + (tile - tiles.sinks) * kTile) + wave * kStep; };
+  auto first_of = [&](int tile) { return tile < tiles.sinks ? tile * kTile : tiles.low + (tile - tiles.sinks) * kTile; };
+  auto first_key = [&](int tile) { return first_of(tile) + wave * kStep; };  // of the wave's own keys
   // A lane's key of a step, and the page that holds it; past the last key the last one's place is asked for.
   auto page_of = [&](int tile) {
     return paged ? table[p.page.quotient((uint32_t)min(first_key(tile) + lane % kStep, any.high - 1))] : 0;
@@ -224,12 +225,12 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
     fetch(keys, key_at, key_words);
   };
   // a step's vectors to the wave's rows in LDS, e4m3 as the elements of T that they stand for
-  auto put = [&](const u32x4 (&words)[kLoads]) {
+  auto put = [&](unsigned char *base, const u32x4 (&words)[kLoads]) {
     __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses are in order)
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
       const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
-      unsigned char *to = held + (wave * kStep + row) * kRow + vector * kLoad * 2;
+      unsigned char *to = base + row * kRow + vector * kLoad * 2;
       if constexpr (kNarrow) {
         u32x4 low, high;
         widened<T>(words[k], &low, &high);
@@ -242,23 +243,24 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
     __builtin_amdgcn_wave_barrier();  // other lanes' rows are read next
   };
 
-  unsigned char *rows = held + wave * kStep * kRow;
+  auto key_rows = [&](int part) { return held + part * kStep * kRow; };
+  auto value_rows = [&](int part) { return held + ((kRowWaves == 1 ? 0 : kWaves) + part) * kStep * kRow; };
   int page = 0;
   if (begin < end) page = page_of(begin);
   // queries: a lane's row is its column, its dims 8 quarter on of every 32
-  u32x4 query[kBlocks][kSteps];
-  AttentionSpan span[kBlocks];
-#pragma unroll
-  for (int n = 0; n < kBlocks; ++n) {
-    const int row = first_row + 16 * n + column, known = min(row, layout.rows - 1), token = (int)p.shared.quotient((uint32_t)known);
+  u32x4 query[kSteps];
+  AttentionSpan span;
+  {
+    const int row = first_row + 16 * row_wave + column, known = min(row, layout.rows - 1), token = (int)p.shared.quotient((uint32_t)known);
     const unsigned char *from = attention_query(p, b, s, chunk.index, token, group * (int)p.shared.divisor + known - token * (int)p.shared.divisor);
-    span[n] = attention_span(p, s.keys, s.first + token);
+    span = attention_span(p, s.keys, s.first + token);
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
-      query[n][k] = u32x4{0, 0, 0, 0};
-      if (row < layout.rows && (kWhole || (4 * k + quarter) * 8 < p.depth)) query[n][k] = load16(from, 4 * k + quarter);
+      query[k] = u32x4{0, 0, 0, 0};
+      if (row < layout.rows && (kWhole || (4 * k + quarter) * 8 < p.depth)) query[k] = load16(from, 4 * k + quarter);
     }
   }
+  if (kRowWaves > 1 && threadIdx.x == 0) no_number = 0;
   if (begin < end) {
     fetch_keys(begin, page);
     fetch(values, value_at, value_words);
@@ -266,174 +268,199 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
   }
   if (p.scale <= 0.0f) {
 #pragma unroll
-    for (int n = 0; n < kBlocks; ++n)
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) query[n][k] = p.scale == 0.0f ? u32x4{0, 0, 0, 0} : query[n][k] ^ 0x80008000u;
+    for (int k = 0; k < kSteps; ++k) query[k] = p.scale == 0.0f ? u32x4{0, 0, 0, 0} : query[k] ^ 0x80008000u;
   }
-  for (int tile = begin; tile < end; ++tile) {
-    const uint32_t these = alive;
-    const int first = first_key(tile);
-    const bool whole = these == 0xFFFFFFFFu && first + kStep <= tile_first.high && first >= tile_last.low;
-
-    put(key_words);
-    __builtin_amdgcn_sched_barrier(0);  // (loads that move up further need registers of their own)
-    if (tile + 1 < end) {
-      fetch_keys(tile + 1, page);
-      if (tile + 2 < end) page = page_of(tile + 2);
+  if (kRowWaves > 1) __syncthreads();  // no_number is cleared
+  // every row of the block sees every key from `first` on
+  auto seen_whole = [&](int first) { return first + kStep <= tile_first.high && first >= tile_last.low; };
+  // keys that are not alive bring zeros
+  auto clear_dead = [&](uint32_t these) {
+    if (these == 0xFFFFFFFFu) return;
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
+      if (((these >> row) & 1u) == 0) value_words[k] = u32x4{0, 0, 0, 0};
     }
-    f32x4 score[kBlocks][2];
+  };
+  // Values that are no numbers, of keys that not every row sees: a weight of 0 would make NaN of them in the product.  They are
+  // added to the rows that see them (a finite weight changes nothing about them) and zeroed.
+  auto add_no_numbers = [&](const unsigned char *from, uint32_t these, int first) {
+#pragma unroll 1
+    for (int j = 0; j < kStep; ++j) {
+      if (((these >> j) & 1u) == 0) continue;
+      const bool sees = attention_sees(p, span, first + j);
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-#pragma unroll
-      for (int n = 0; n < kBlocks; ++n) score[n][sub] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(rows + (16 * sub + column) * kRow + (4 * k + quarter) * 16);
-#pragma unroll
-        for (int n = 0; n < kBlocks; ++n) score[n][sub] = product16<T>(w, query[n][k], score[n][sub]);
-      }
-    }
-    if (!whole) {
-#pragma unroll
-      for (int n = 0; n < kBlocks; ++n)
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = 16 * sub + 4 * quarter + r;
-            if (((these >> j) & 1u) == 0 || !attention_sees(p, span[n], first + j)) score[n][sub][r] = -INFINITY;
-          }
-    }
-    float most[kBlocks];
-    bool grown = false;
-#pragma unroll
-    for (int n = 0; n < kBlocks; ++n) {
-      most[n] = fmaxf(fmaxf(fmaxf(score[n][0][0], score[n][0][1]), fmaxf(score[n][0][2], score[n][0][3])),
-                      fmaxf(fmaxf(score[n][1][0], score[n][1][1]), fmaxf(score[n][1][2], score[n][1][3])));
-      most[n] = rows_max(most[n]) * c;
-      grown |= most[n] > top[n] + kSlack;
-    }
-    if (__ballot(grown) != 0) {
-#pragma unroll
-      for (int n = 0; n < kBlocks; ++n) {
-        const float next = fmaxf(top[n], most[n]);
-        const float keep = top[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[n] - next);
-        top[n] = next;
-        sum[n] *= keep;
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) out[n][d] *= keep;
-      }
-    }
-    u32x4 weights[kBlocks];
-#pragma unroll
-    for (int n = 0; n < kBlocks; ++n) {
-      const float shift = top[n] == -INFINITY ? 0.0f : top[n];
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
+      for (int d = 0; d < kDims; ++d) {
+        float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          score[n][sub][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[n][sub][r], c, -shift));
-          sum[n] += score[n][sub][r];
+          const float x = Traits<T>::load(from + j * kRow, 16 * d + 4 * quarter + r);
+          v[r] = fabsf(x) < INFINITY ? 0.0f : x;
         }
-        weights[n][2 * sub] = pack2<T>(score[n][sub][0], score[n][sub][1]);
-        weights[n][2 * sub + 1] = pack2<T>(score[n][sub][2], score[n][sub][3]);
+        if (sees) out[d] += f32x4{v[0], v[1], v[2], v[3]};
+        asm volatile("" : : : "memory");  // (a dim at a time: all at once would cost every step its registers)
       }
     }
+  };
+  auto any_no_number = [&]() {
+    uint32_t found = 0;
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) found |= no_numbers<C>(value_words[k]);
+    return __ballot(found != 0) != 0;
+  };
+  auto keep_numbers = [&]() {
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) value_words[k] = numbers_only<C>(value_words[k]);
+  };
 
-    // keys that are not alive bring zeros
-    if (these != 0xFFFFFFFFu) {
-#pragma unroll
-      for (int k = 0; k < kLoads; ++k) {
-        const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
-        if (((these >> row) & 1u) == 0) value_words[k] = u32x4{0, 0, 0, 0};
+  for (int tile = begin; tile < end; ++tile) {
+    const uint32_t own = alive;
+    put(key_rows(wave), key_words);
+    if constexpr (kRowWaves == 1) {
+      __builtin_amdgcn_sched_barrier(0);  // (loads that move up further need registers of their own)
+      if (tile + 1 < end) {
+        fetch_keys(tile + 1, page);
+        if (tile + 2 < end) page = page_of(tile + 2);
       }
-    }
-    if (!whole && s.rows > 1) {
-      // Values that are no numbers, of keys that not every row sees: a weight of 0 would make NaN of them in the product.
-      // They are added to the rows that see them (a finite weight changes nothing about them) and zeroed.
-      uint32_t found = 0;
-#pragma unroll
-      for (int k = 0; k < kLoads; ++k) found |= no_numbers<C>(value_words[k]);
-      if (__ballot(found != 0) != 0) {
-        put(value_words);
-        for (int j = 0; j < kStep; ++j) {
-          if (((these >> j) & 1u) == 0) continue;
-#pragma unroll
-          for (int d = 0; d < kDims; ++d) {
-            float v[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float x = Traits<T>::load(rows + j * kRow, 16 * d + 4 * quarter + r);
-              v[r] = fabsf(x) < INFINITY ? 0.0f : x;
-            }
-#pragma unroll
-            for (int n = 0; n < kBlocks; ++n)
-              if (attention_sees(p, span[n], first + j)) out[n][d] += f32x4{v[0], v[1], v[2], v[3]};
-            asm volatile("" : : : "memory");  // (a dim at a time: all at once would cost every step its registers)
-          }
+    } else {
+      clear_dead(own);
+      if (lane == 0) shared_alive[wave] = own;
+      const bool odd = s.rows > 1 && !(own == 0xFFFFFFFFu && seen_whole(first_key(tile))) && any_no_number();
+      if (odd && lane == 0) no_number = tile + 1;
+      put(value_rows(wave), value_words);
+      __syncthreads();
+      if (no_number == tile + 1) {
+#pragma unroll 1
+        for (int sub = 0; sub < kRowWaves; ++sub) {
+          const int part = key_group * kRowWaves + sub;
+          add_no_numbers(value_rows(part), shared_alive[part], first_of(tile) + part * kStep);
         }
-#pragma unroll
-        for (int k = 0; k < kLoads; ++k) value_words[k] = numbers_only<C>(value_words[k]);
+        __syncthreads();
+        keep_numbers();
+        put(value_rows(wave), value_words);
+        __syncthreads();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (tile + 1 < end) {
+        fetch_keys(tile + 1, page);
+        if (tile + 2 < end) page = page_of(tile + 2);
+        fetch(values, value_at, value_words);
       }
     }
-    put(value_words);
-    __builtin_amdgcn_sched_barrier(0);
-    if (tile + 1 < end) fetch(values, value_at, value_words);
+#pragma unroll 1
+    for (int sub = 0; sub < kRowWaves; ++sub) {
+      const int part = kRowWaves == 1 ? wave : key_group * kRowWaves + sub, first = first_of(tile) + part * kStep;
+      const uint32_t these = kRowWaves == 1 ? own : (uint32_t)__builtin_amdgcn_readfirstlane((int)shared_alive[part]);
+      const bool whole = these == 0xFFFFFFFFu && seen_whole(first);
+      f32x4 score[2];
+      const unsigned char *from = key_rows(part);
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) {
-      const unsigned char *at = rows + (4 * quarter + column / 4) * kRow + (d * 16 + column % 4 * 4) * 2;
-      const uint2 near = read_transposed(at), far = read_transposed(at + 16 * kRow);
-      const u32x4 value = {near.x, near.y, far.x, far.y};
+      for (int half = 0; half < 2; ++half) {
+        score[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int n = 0; n < kBlocks; ++n) out[n][d] = product16<T>(value, weights[n], out[n][d]);
+        for (int k = 0; k < kSteps; ++k) {
+          const u32x4 w = *reinterpret_cast<const u32x4 *>(from + (16 * half + column) * kRow + (4 * k + quarter) * 16);
+          score[half] = product16<T>(w, query[k], score[half]);
+        }
+      }
+      if (!whole) {
+        asm volatile("" : : : "memory");  // (a branch: as selects, the comparisons are every step's)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = 16 * half + 4 * quarter + r;
+            if (((these >> j) & 1u) == 0 || !attention_sees(p, span, first + j)) score[half][r] = -INFINITY;
+          }
+      }
+      const float most = rows_max(fmaxf(fmaxf(fmaxf(score[0][0], score[0][1]), fmaxf(score[0][2], score[0][3])),
+                                        fmaxf(fmaxf(score[1][0], score[1][1]), fmaxf(score[1][2], score[1][3])))) *
+                         c;
+      if (__ballot(most > top + kSlack) != 0) {
+        const float next = fmaxf(top, most);
+        const float keep = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - next);  // (what there is without a maximum is zeros and what is no number)
+        top = next;
+        sum *= keep;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) out[d] *= keep;
+      }
+      u32x4 weights;
+      const float shift = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          score[half][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[half][r], c, -shift));
+          sum += score[half][r];
+        }
+        weights[2 * half] = pack2<T>(score[half][0], score[half][1]);
+        weights[2 * half + 1] = pack2<T>(score[half][2], score[half][3]);
+      }
+      if constexpr (kRowWaves == 1) {
+        clear_dead(these);
+        if (!whole && s.rows > 1 && any_no_number()) {
+          put(value_rows(wave), value_words);
+          add_no_numbers(value_rows(wave), these, first);
+          keep_numbers();
+        }
+        put(value_rows(wave), value_words);
+        __builtin_amdgcn_sched_barrier(0);
+        if (tile + 1 < end) fetch(values, value_at, value_words);
+      }
+      from = value_rows(part);
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) {
+        const unsigned char *at = from + (4 * quarter + column / 4) * kRow + (d * 16 + column % 4 * 4) * 2;
+        const uint2 near = read_transposed(at), far = read_transposed(at + 16 * kRow);
+        const u32x4 value = {near.x, near.y, far.x, far.y};
+        out[d] = product16<T>(value, weights, out[d]);
+      }
     }
+    if (kRowWaves > 1) __syncthreads();  // the rows in LDS are read
   }
 
-  // join the waves, 16 rows at a time
+  // join the waves of the same rows
   float *joined = reinterpret_cast<float *>(held);
-  const int join_row = (int)threadIdx.x / 16;
+  constexpr int kRowThreads = 16 / kRowWaves;  // threads of a row
+  const int join_row = (int)threadIdx.x / kRowThreads, join_wave = join_row / 16, join_column = join_row % 16;
+  __syncthreads();
+  const float total = rows_sum(sum);
+  if (quarter == 0) joined_top[wave][column] = top, joined_sum[wave][column] = total;
 #pragma unroll
-  for (int n = 0; n < kBlocks; ++n) {
-    __syncthreads();
-    const float total = rows_sum(sum[n]);
-    if (quarter == 0) joined_top[wave][column] = top[n], joined_sum[wave][column] = total;
+  for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4 *>(joined + (wave * 16 + column) * kJoinRow + d * 16 + 4 * quarter) = out[d];
+  __syncthreads();
+  const int row = first_row + join_row;
+  if (row >= layout.rows) return;
+  float most = joined_top[join_wave][join_column];
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4 *>(joined + (wave * 16 + column) * kJoinRow + d * 16 + 4 * quarter) = out[n][d];
-    __syncthreads();
-    const int row = first_row + 16 * n + join_row;
-    if (row < layout.rows) {
-      float most = joined_top[0][join_row];
+  for (int g = 1; g < kGroups; ++g) most = fmaxf(most, joined_top[g * kRowWaves + join_wave][join_column]);
+  const float shift = most == -INFINITY ? 0.0f : most;
+  float keep[kGroups], all = 0.0f;
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) most = fmaxf(most, joined_top[w][join_row]);
-      const float shift = most == -INFINITY ? 0.0f : most;
-      float keep[kWaves], all = 0.0f;
+  for (int g = 0; g < kGroups; ++g) {
+    keep[g] = __builtin_amdgcn_exp2f(joined_top[g * kRowWaves + join_wave][join_column] - shift);
+    all += joined_sum[g * kRowWaves + join_wave][join_column] * keep[g];
+  }
+  const int token = (int)p.shared.quotient((uint32_t)row);
+  const int64_t at = (s.row + token) * p.queries + group * (int)p.shared.divisor + row - token * (int)p.shared.divisor;
+  const int64_t part = ((int64_t)slot * p.heads + group) * layout.rows + row;
+  const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
+  for (int d = (int)threadIdx.x % kRowThreads * 4; d < p.depth; d += kRowThreads * 4) {
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        keep[w] = __builtin_amdgcn_exp2f(joined_top[w][join_row] - shift);
-        all += joined_sum[w][join_row] * keep[w];
-      }
-      const int token = (int)p.shared.quotient((uint32_t)row);
-      const int64_t at = (s.row + token) * p.queries + group * (int)p.shared.divisor + row - token * (int)p.shared.divisor;
-      const int64_t part = ((int64_t)slot * p.heads + group) * layout.rows + row;
-      const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
-      for (int d = (int)threadIdx.x % 16 * 4; d < p.depth; d += 64) {
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) o += *reinterpret_cast<const f32x4 *>(joined + (w * 16 + join_row) * kJoinRow + d) * keep[w];
-        if (chunk.chunks == 1) {
-          uint2 w;
-          w.x = pack2<T>(o[0] * inverse, o[1] * inverse);
-          w.y = pack2<T>(o[2] * inverse, o[3] * inverse);
-          *reinterpret_cast<uint2 *>(static_cast<unsigned char *>(b.out) + (at * p.depth + d) * 2) = w;
-        } else {
-          *reinterpret_cast<f32x4 *>(layout.partial + part * p.depth + d) = o;
-        }
-      }
-      if (threadIdx.x % 16 == 0) {
-        if (chunk.chunks != 1) layout.stats[part] = float2{most, all};
-        else if (b.logs != nullptr) b.logs[at] = all == 0.0f ? -INFINITY : (most + __builtin_amdgcn_logf(all)) * kLn2;
-      }
+    for (int g = 0; g < kGroups; ++g) o += *reinterpret_cast<const f32x4 *>(joined + ((g * kRowWaves + join_wave) * 16 + join_column) * kJoinRow + d) * keep[g];
+    if (chunk.chunks == 1) {
+      uint2 w;
+      w.x = pack2<T>(o[0] * inverse, o[1] * inverse);
+      w.y = pack2<T>(o[2] * inverse, o[3] * inverse);
+      *reinterpret_cast<uint2 *>(static_cast<unsigned char *>(b.out) + (at * p.depth + d) * 2) = w;
+    } else {
+      *reinterpret_cast<f32x4 *>(layout.partial + part * p.depth + d) = o;
     }
+  }
+  if (threadIdx.x % kRowThreads == 0) {
+    if (chunk.chunks != 1) layout.stats[part] = float2{most, all};
+    else if (b.logs != nullptr) b.logs[at] = all == 0.0f ? -INFINITY : (most + __builtin_amdgcn_logf(all)) * kLn2;
   }
 }
 
@@ -486,9 +513,9 @@ __global__ __launch_bounds__(join_threads(kDepth)) void attention_join(Attention
 
 }  // namespace
 
-template <class C, int kDepth, int kBlocks, bool kWhole> struct AttentionSplitTag {
+template <class C, int kDepth, int kRowWaves, bool kWhole> struct AttentionSplitTag {
   static std::string text() {
-    return std::string("attention_split/") + (std::is_same<C, E4M3>::value ? "e4m3/" : "") + (kWhole ? "d" : "below-d") + std::to_string(kDepth) + "/" + std::to_string(16 * kBlocks) + "-rows";
+    return std::string("attention_split/") + (std::is_same<C, E4M3>::value ? "e4m3/" : "") + (kWhole ? "d" : "below-d") + std::to_string(kDepth) + "/" + std::to_string(16 * kRowWaves) + "-rows";
   }
 };
 template <int kDepth> struct AttentionJoinTag {
@@ -497,12 +524,12 @@ template <int kDepth> struct AttentionJoinTag {
 
 namespace {
 int padded_depth(const AttentionParams &p) { return p.depth <= 64 ? 64 : p.depth <= 128 ? 128 : 256; }
-int blocks_of(const AttentionParams &p) {
+int row_waves_of(const AttentionParams &p) {
   const int64_t rows = (int64_t)p.rows * p.shared.divisor;
-  return rows <= 16 ? 1 : rows <= 32 || p.depth > 128 ? 2 : 4;
+  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
 }
 int row_tiles_of(const AttentionParams &p) {
-  const int64_t each = 16 * blocks_of(p);
+  const int64_t each = 16 * row_waves_of(p);
   return (int)(((int64_t)p.rows * p.shared.divisor + each - 1) / each);
 }
 }  // namespace
@@ -512,7 +539,7 @@ AttentionSplit attention_split_of(const AttentionParams &p, int compute_units) {
   // The chunks of one key head and tile of rows: three rounds of the blocks that the device holds, so that the last ones of
   // ragged sequences leave it idle for a third of a block.
   const int64_t lanes = (int64_t)p.heads * row_tiles_of(p);
-  const int64_t blocks = (int64_t)compute_units * resident(p.narrow_cache, padded_depth(p), blocks_of(p));
+  const int64_t blocks = (int64_t)compute_units * resident(p.narrow_cache, padded_depth(p), row_waves_of(p));
   const int64_t target = (3 * blocks + lanes - 1) / lanes;
   split.blocks = (int)((blocks + lanes - 1) / lanes);
   // tiles of a sequence: of all its keys, or of the window of its new tokens and the sinks
@@ -543,37 +570,34 @@ bool attention_split_serves(Elem type, const AttentionParams &p, bool vector_ali
 }
 
 namespace {
-template <class T, class C, int kDepth, int kBlocks>
+template <class T, class C, int kDepth, int kRowWaves>
 void start_split(const AttentionParams &p, const AttentionBuffers &b, const SplitLayout &layout, const AttentionSplit &split, hipStream_t stream) {
   const dim3 grid((uint32_t)split.slots * layout.lanes.divisor), block(kThreads);
   if (p.depth == kDepth) {
-    note_variant<AttentionSplitTag<C, kDepth, kBlocks, true>>();
-    hipLaunchKernelGGL((attention_split<T, C, kDepth, kBlocks, true>), grid, block, 0, stream, p, b, layout);
+    note_variant<AttentionSplitTag<C, kDepth, kRowWaves, true>>();
+    hipLaunchKernelGGL((attention_split<T, C, kDepth, kRowWaves, true>), grid, block, 0, stream, p, b, layout);
   } else {
-    note_variant<AttentionSplitTag<C, kDepth, kBlocks, false>>();
-    hipLaunchKernelGGL((attention_split<T, C, kDepth, kBlocks, false>), grid, block, 0, stream, p, b, layout);
+    note_variant<AttentionSplitTag<C, kDepth, kRowWaves, false>>();
+    hipLaunchKernelGGL((attention_split<T, C, kDepth, kRowWaves, false>), grid, block, 0, stream, p, b, layout);
   }
   if (!split.joined) return;
   note_variant<AttentionJoinTag<kDepth>>();
   hipLaunchKernelGGL((attention_join<T, kDepth>), dim3(layout.lines.divisor * (uint32_t)p.sequences), dim3(join_threads(kDepth)), 0, stream, p, b, layout);
 }
+template <class T, class C, int kDepth>
+void split_by_rows(const AttentionParams &p, const AttentionBuffers &b, const SplitLayout &layout, const AttentionSplit &split, hipStream_t stream) {
+  switch (row_waves_of(p)) {
+    case 1: start_split<T, C, kDepth, 1>(p, b, layout, split, stream); break;
+    case 2: start_split<T, C, kDepth, 2>(p, b, layout, split, stream); break;
+    default: start_split<T, C, kDepth, 4>(p, b, layout, split, stream);
+  }
+}
 template <class T, class C>
 void split_by_depth(const AttentionParams &p, const AttentionBuffers &b, const SplitLayout &layout, const AttentionSplit &split, hipStream_t stream) {
-  const int blocks = blocks_of(p);
   switch (padded_depth(p)) {
-    case 64:
-      if (blocks == 1) start_split<T, C, 64, 1>(p, b, layout, split, stream);
-      else if (blocks == 2) start_split<T, C, 64, 2>(p, b, layout, split, stream);
-      else start_split<T, C, 64, 4>(p, b, layout, split, stream);
-      break;
-    case 128:
-      if (blocks == 1) start_split<T, C, 128, 1>(p, b, layout, split, stream);
-      else if (blocks == 2) start_split<T, C, 128, 2>(p, b, layout, split, stream);
-      else start_split<T, C, 128, 4>(p, b, layout, split, stream);
-      break;
-    default:
-      if (blocks == 1) start_split<T, C, 256, 1>(p, b, layout, split, stream);
-      else start_split<T, C, 256, 2>(p, b, layout, split, stream);
+    case 64: split_by_rows<T, C, 64>(p, b, layout, split, stream); break;
+    case 128: split_by_rows<T, C, 128>(p, b, layout, split, stream); break;
+    default: split_by_rows<T, C, 256>(p, b, layout, split, stream);
   }
 }
 }  // namespace

@@ -414,7 +414,7 @@ bool attention_split_serves(Elem type, const AttentionParams &p, bool vector_ali
 hipError_t launch_attention_split(Elem type, const AttentionParams &p, const AttentionBuffers &b, const AttentionSplit &split, void *workspace,
                                   hipStream_t stream);
 bool attention_tiles_serves(Elem type, const AttentionParams &p, bool vector_aligned);
-hipError_t launch_attention_tiles(Elem type, const AttentionParams &p, const AttentionBuffers &b, hipStream_t stream);
+hipError_t launch_attention_tiles(Elem type, const AttentionParams &p, const AttentionBuffers &b, int compute_units, hipStream_t stream);
 hipError_t launch_attention_general(Elem type, const AttentionParams &p, const AttentionBuffers &b, hipStream_t stream);
 
 // PagedAppend: rows of [tokens, heads, depth] keys and values to their slots of a dense cache.

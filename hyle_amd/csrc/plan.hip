@@ -2094,7 +2094,7 @@ hyle_hip_status hyle_hip_plan_launch(const hyle_hip_plan *plan, const void *cons
       const bool vectors = aligned(inputs[0], 16) && aligned(inputs[1], 16) && aligned(b.value, 16) && aligned(b.out, 16);
       if (plan->attention_few_rows && attention_split_serves(plan->elem, plan->attention, vectors))
         err = launch_attention_split(plan->elem, plan->attention, b, plan->attention_split, workspace, stream);
-      else if (attention_tiles_serves(plan->elem, plan->attention, vectors)) err = launch_attention_tiles(plan->elem, plan->attention, b, stream);
+      else if (attention_tiles_serves(plan->elem, plan->attention, vectors)) err = launch_attention_tiles(plan->elem, plan->attention, b, plan->context->compute_units, stream);
       else err = launch_attention_general(plan->elem, plan->attention, b, stream);
       break;
     }
