@@ -18,15 +18,15 @@ namespace {
 constexpr int kWaves = 4, kThreads = kWaves * kWaveLanes;
 constexpr int kStep = 32, kTile = kWaves * kStep;  // keys of a wave's step and of a block's
 
-// How a sequence's tiles are dealt: `tiles` of them, the first `sinks` of which hold the sinks before the window's first key
-// `low` (rounded down to a tile).
+// How a sequence's tiles are dealt: `tiles` of them, the first `sinks` of which hold the sinks before `low`, the window's first key
+// (rounded down to a wave's step).
 struct SplitTiles {
   int low, sinks, tiles;
 };
 __device__ __forceinline__ SplitTiles tiles_of(const AttentionParams &p, const AttentionSequence &s) {
   const AttentionSpan first = attention_span(p, s.keys, s.first), last = attention_span(p, s.keys, s.first + s.rows - 1);
   SplitTiles t;
-  t.low = min(first.low, last.high) / kTile * kTile;
+  t.low = min(first.low, last.high) / kStep * kStep;
   t.sinks = (min(min(p.sinks, t.low), last.high) + kTile - 1) / kTile;
   t.tiles = t.sinks + (last.high - t.low + kTile - 1) / kTile;
   return t;
@@ -56,6 +56,12 @@ __device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t
     if (slot >= p.sequences) return false;
     *c = SplitChunk{slot, 0, 1, slot, 1 << 24, __builtin_amdgcn_readfirstlane(attention_mark(p, marks, slot))};
     return true;
+  }
+  if (p.sequences == 1) {
+    const int mark = __builtin_amdgcn_readfirstlane(attention_mark(p, marks, 0)), tiles = tiles_of(p, attention_sequence_of(p, 0, mark)).tiles;
+    const int each = max((int)(((uint32_t)tiles + (uint32_t)target - 1) / (uint32_t)target), tiles > blocks ? 2 : 1);
+    *c = SplitChunk{0, slot, max(1, (tiles + each - 1) / each), 0, each, mark};
+    return slot < c->chunks;
   }
   auto tiles_at = [&](int index, int mark) { return index < p.sequences ? (uint32_t)tiles_of(p, attention_sequence_of(p, index, mark)).tiles : 0u; };
   const int first_mark = attention_mark(p, marks, min(lane, p.sequences - 1));
@@ -210,7 +216,7 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
   };
   auto fetch_keys = [&](int tile, int page) {
     const int key = first_key(tile) + lane % kStep, known = min(key, any.high - 1);
-    bool there = attention_sees(p, any, key);
+    bool there = attention_sees(p, any, key) && (tile >= tiles.sinks || key < tiles.low);
     int64_t key_at;
     if (paged) {
       there = there && (uint32_t)page < (uint32_t)p.pages;
@@ -224,6 +230,7 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
     alive = (uint32_t)__ballot(there);
     fetch(keys, key_at, key_words);
   };
+  auto fetch_values = [&]() { fetch(values, value_at, value_words); };
   // a step's vectors to the wave's rows in LDS, e4m3 as the elements of T that they stand for
   auto put = [&](unsigned char *base, const u32x4 (&words)[kLoads]) {
     __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses are in order)
@@ -263,7 +270,7 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
   if (kRowWaves > 1 && threadIdx.x == 0) no_number = 0;
   if (begin < end) {
     fetch_keys(begin, page);
-    fetch(values, value_at, value_words);
+    fetch_values();
     if (begin + 1 < end) page = page_of(begin + 1);
   }
   if (p.scale <= 0.0f) {
@@ -344,7 +351,7 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
       if (tile + 1 < end) {
         fetch_keys(tile + 1, page);
         if (tile + 2 < end) page = page_of(tile + 2);
-        fetch(values, value_at, value_words);
+        fetch_values();
       }
     }
 #pragma unroll 1
@@ -405,7 +412,7 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
         }
         put(value_rows(wave), value_words);
         __builtin_amdgcn_sched_barrier(0);
-        if (tile + 1 < end) fetch(values, value_at, value_words);
+        if (tile + 1 < end) fetch_values();
       }
       from = value_rows(part);
 #pragma unroll
@@ -464,23 +471,24 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
   }
 }
 
-constexpr int join_threads(int depth) { return depth == 256 ? 512 : 256; }
-// The chunks of one query row joined: four dims to a thread, kParts chunks side by side.
-template <class T, int kDepth>
-__global__ __launch_bounds__(join_threads(kDepth)) void attention_join(AttentionParams p, AttentionBuffers b, SplitLayout layout) {
-  constexpr int kLanes = kDepth / 4, kParts = join_threads(kDepth) / kLanes;
-  __shared__ __attribute__((aligned(16))) f32x4 joined[kParts][kLanes];
-  __shared__ float sums[kParts];
-  const int index = (int)layout.lines.quotient(blockIdx.x), rest = (int)blockIdx.x - index * (int)layout.lines.divisor;  // key head and row
+// The chunks of a query row joined, four dims to a thread.  kSide: kParts chunks side by side, a row to a block, for few rows of
+// many chunks; otherwise a row to kLanes threads.
+constexpr int join_threads(int depth, bool side) { return side && depth == 256 ? 512 : 256; }
+template <class T, int kDepth, bool kSide>
+__global__ __launch_bounds__(join_threads(kDepth, kSide)) void attention_join(AttentionParams p, AttentionBuffers b, SplitLayout layout) {
+  constexpr int kLanes = kDepth / 4, kParts = kSide ? join_threads(kDepth, kSide) / kLanes : 1, kRows = kSide ? 1 : join_threads(kDepth, kSide) / kLanes;
+  const uint32_t line = blockIdx.x * kRows + (kSide ? 0u : threadIdx.x / kLanes);
+  const int index = (int)layout.lines.quotient(line), rest = (int)line - index * (int)layout.lines.divisor;  // key head and row
+  if (!kSide && index >= p.sequences) return;
   const int2 place = layout.places[index];
   if (place.y == 1) return;  // the split kernel's block was the whole sequence
   const int64_t stride = (int64_t)p.heads * layout.rows, first = (int64_t)place.x * stride + rest;
-  const int lane = (int)threadIdx.x % kWaveLanes;
-  float most = -INFINITY;  // every wave looks at all chunks' maxima
-  for (int i = lane; i < place.y; i += kWaveLanes) most = fmaxf(most, layout.stats[first + i * stride].x);
-  most = group_max<kWaveLanes>(most);
+  const int lane = (int)threadIdx.x % (kSide ? kWaveLanes : kLanes);
+  float most = -INFINITY;  // every wave, or row, looks at all chunks' maxima
+  for (int i = lane; i < place.y; i += kSide ? kWaveLanes : kLanes) most = fmaxf(most, layout.stats[first + i * stride].x);
+  most = group_max<kSide ? kWaveLanes : kLanes>(most);
   const float shift = most == -INFINITY ? 0.0f : most;
-  const int dim = (int)threadIdx.x % kLanes * 4, part = (int)threadIdx.x / kLanes;
+  const int dim = (int)threadIdx.x % kLanes * 4, part = kSide ? (int)threadIdx.x / kLanes : 0;
   f32x4 out = {0.0f, 0.0f, 0.0f, 0.0f};
   float sum = 0.0f;
   const bool has = dim < p.depth;
@@ -493,12 +501,16 @@ __global__ __launch_bounds__(join_threads(kDepth)) void attention_join(Attention
 #pragma unroll
     for (int e = 0; e < 4; ++e) out[e] = __builtin_fmaf(o[e], keep, out[e]);
   }
-  joined[part][dim / 4] = out;
-  if (dim == 0) sums[part] = sum;
-  __syncthreads();
-  if (part != 0) return;
+  if constexpr (kSide) {
+    __shared__ __attribute__((aligned(16))) f32x4 joined[kParts][kLanes];
+    __shared__ float sums[kParts];
+    joined[part][dim / 4] = out;
+    if (dim == 0) sums[part] = sum;
+    __syncthreads();
+    if (part != 0) return;
 #pragma unroll
-  for (int i = 1; i < kParts; ++i) out += joined[i][dim / 4], sum += sums[i];
+    for (int i = 1; i < kParts; ++i) out += joined[i][dim / 4], sum += sums[i];
+  }
   const int group = rest / layout.rows, row = rest - group * layout.rows, token = (int)p.shared.quotient((uint32_t)row);
   const int64_t at = ((int64_t)index * p.rows + token) * p.queries + group * (int)p.shared.divisor + row - token * (int)p.shared.divisor;
   if (has) {
@@ -518,8 +530,8 @@ template <class C, int kDepth, int kRowWaves, bool kWhole> struct AttentionSplit
     return std::string("attention_split/") + (std::is_same<C, E4M3>::value ? "e4m3/" : "") + (kWhole ? "d" : "below-d") + std::to_string(kDepth) + "/" + std::to_string(16 * kRowWaves) + "-rows";
   }
 };
-template <int kDepth> struct AttentionJoinTag {
-  static std::string text() { return "attention_join/d" + std::to_string(kDepth); }
+template <int kDepth, bool kSide> struct AttentionJoinTag {
+  static std::string text() { return "attention_join/d" + std::to_string(kDepth) + (kSide ? "/row-to-block" : "/rows"); }
 };
 
 namespace {
@@ -534,6 +546,9 @@ int row_tiles_of(const AttentionParams &p) {
 }
 }  // namespace
 
+// Sequences of so few tiles are not split: a tile takes a block about 1 us, the second kernel 4.
+constexpr int kUnsplit = 4;
+
 AttentionSplit attention_split_of(const AttentionParams &p, int compute_units) {
   AttentionSplit split;
   // The chunks of one key head and tile of rows: three rounds of the blocks that the device holds, so that the last ones of
@@ -545,7 +560,7 @@ AttentionSplit attention_split_of(const AttentionParams &p, int compute_units) {
   // tiles of a sequence: of all its keys, or of the window of its new tokens and the sinks
   int64_t most = ((int64_t)p.keys + kTile - 1) / kTile;
   if (p.window != 0) {
-    const int64_t seen = ((int64_t)p.window + p.rows + kTile - 1) / kTile + 1 + ((int64_t)p.sinks + kTile - 1) / kTile;
+    const int64_t seen = ((int64_t)p.window + p.rows + kStep + kTile - 1) / kTile + ((int64_t)p.sinks + kTile - 1) / kTile;
     if (seen < most) most = seen;
   }
   split.target = (int)target;
@@ -555,7 +570,7 @@ AttentionSplit attention_split_of(const AttentionParams &p, int compute_units) {
   if (target < slots) slots = target;
   slots += p.sequences;
   split.slots = (int)slots;
-  split.joined = p.keys > kTile && target > 1;
+  split.joined = most > kUnsplit && target > 1;
   if (!split.joined) split.target = 0, split.slots = p.sequences;
   const int64_t rows = (int64_t)p.rows * p.shared.divisor * p.heads * split.slots;
   split.stats_offset = ((size_t)rows * (size_t)p.depth * sizeof(float) + 255) / 256 * 256;
@@ -581,8 +596,15 @@ void start_split(const AttentionParams &p, const AttentionBuffers &b, const Spli
     hipLaunchKernelGGL((attention_split<T, C, kDepth, kRowWaves, false>), grid, block, 0, stream, p, b, layout);
   }
   if (!split.joined) return;
-  note_variant<AttentionJoinTag<kDepth>>();
-  hipLaunchKernelGGL((attention_join<T, kDepth>), dim3(layout.lines.divisor * (uint32_t)p.sequences), dim3(join_threads(kDepth)), 0, stream, p, b, layout);
+  const uint32_t lines = layout.lines.divisor * (uint32_t)p.sequences;
+  if (lines <= 2048) {
+    note_variant<AttentionJoinTag<kDepth, true>>();
+    hipLaunchKernelGGL((attention_join<T, kDepth, true>), dim3(lines), dim3(join_threads(kDepth, true)), 0, stream, p, b, layout);
+  } else {
+    constexpr uint32_t kRows = join_threads(kDepth, false) / (kDepth / 4);
+    note_variant<AttentionJoinTag<kDepth, false>>();
+    hipLaunchKernelGGL((attention_join<T, kDepth, false>), dim3((lines + kRows - 1) / kRows), dim3(join_threads(kDepth, false)), 0, stream, p, b, layout);
+  }
 }
 template <class T, class C, int kDepth>
 void split_by_rows(const AttentionParams &p, const AttentionBuffers &b, const SplitLayout &layout, const AttentionSplit &split, hipStream_t stream) {
