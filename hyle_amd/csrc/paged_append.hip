@@ -1,7 +1,7 @@
 // paged_append.hip -- keys and values of new tokens to their slots of a paged cache [pages, 2, heads, page, depth].
 //
-// A thread moves eight elements of a head (16 bytes of f16 / bf16, 8 of e4m3) or, where a row is not made of whole aligned
-// vectors, one.  Bound by bytes: every element is read once and written once.
+// A thread moves eight elements of a head (16 bytes of f16 / bf16), sixteen for a cache of e4m3 where the depth allows, or, where
+// a row is not made of whole aligned vectors, one.  Bound by bytes: every element is read once and written once.
 #include "attention.h"
 
 namespace hyle_hip {
@@ -57,10 +57,11 @@ __global__ __launch_bounds__(kBlockThreads) void paged_append(AppendLayout p, co
 #pragma unroll
         for (int e = 0; e < Traits<T>::kVec; ++e) x[v * Traits<T>::kVec + e] = part[e];
       }
-      uint2 packed;
-      packed.x = pack_e4m3(x[0], x[1], x[2], x[3]);
-      packed.y = pack_e4m3(x[4], x[5], x[6], x[7]);
-      *reinterpret_cast<uint2 *>(cache + to) = packed;
+      uint32_t packed[kElements / 4];
+#pragma unroll
+      for (int e = 0; e < kElements / 4; ++e) packed[e] = pack_e4m3(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+      if constexpr (kElements == 16) store16(cache + to, 0, u32x4{packed[0], packed[1], packed[2], packed[3]});
+      else *reinterpret_cast<uint2 *>(cache + to) = uint2{packed[0], packed[1]};
     } else {
 #pragma unroll
       for (int v = 0; v < kVectors; ++v) store16(cache + to * Traits<T>::kSize, v, w[v]);
@@ -70,14 +71,14 @@ __global__ __launch_bounds__(kBlockThreads) void paged_append(AppendLayout p, co
 
 }  // namespace
 
-template <bool kNarrow, bool kVector> struct AppendTag {
-  static std::string text() { return std::string("paged_append/") + (kNarrow ? "e4m3/" : "kept/") + (kVector ? "vectors" : "elements"); }
+template <bool kNarrow, int kElements> struct AppendTag {
+  static std::string text() { return std::string("paged_append/") + (kNarrow ? "e4m3/" : "kept/") + std::to_string(kElements); }
 };
 
 template <class T, bool kNarrow, int kElements>
 static void start(AppendLayout layout, const AppendParams &p, const void *keys, const void *values, const int32_t *slots, void *cache,
                   hipStream_t stream) {
-  note_variant<AppendTag<kNarrow, kElements != 1>>();
+  note_variant<AppendTag<kNarrow, kElements>>();
   const uint32_t units = p.depth / kElements;
   layout.units = 2 * p.heads * units;
   layout.unit = Divisor(layout.units);
@@ -100,7 +101,8 @@ hipError_t launch_paged_append(Elem type, const AppendParams &p, const void *key
   auto chosen = [&](auto tag, auto narrow) {
     using T = decltype(tag);
     constexpr bool kNarrow = decltype(narrow)::value;
-    if (vectors) start<T, kNarrow, 8>(layout, p, keys, values, slots, cache, stream);
+    if (vectors && kNarrow && p.depth % 16 == 0) start<T, kNarrow, kNarrow ? 16 : 8>(layout, p, keys, values, slots, cache, stream);
+    else if (vectors) start<T, kNarrow, 8>(layout, p, keys, values, slots, cache, stream);
     else start<T, kNarrow, 1>(layout, p, keys, values, slots, cache, stream);
   };
   auto typed = [&](auto tag) { p.narrow_cache ? chosen(tag, std::true_type{}) : chosen(tag, std::false_type{}); };

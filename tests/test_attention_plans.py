@@ -111,3 +111,16 @@ def test_no_operand_may_be_an_output():
     assert not any(plan.alias_support(0, i) for i in range(3))
     append = hc.prepare(CTX, hc.PagedAppend(10, 16, BF16), D(BF16, [3, 4, 64]), D(BF16, [3, 4, 64]), D(I32, [3]))
     assert not any(append.alias_support(0, i) for i in range(3))
+
+
+def test_workspaces_hold_what_split_keys_leave():
+    def plan(sequences, columns, window=0, depth=128):
+        return hc.prepare(CTX, hc.PagedAttention(window=window), D(BF16, [sequences, 8, depth]), D(BF16, [64, 2, 2, 16, depth]), D(I32, [sequences, columns]),
+                          D(I32, [sequences]))
+    short = plan(4, 32)                       # 512 keys: a block to a sequence and key head
+    assert short.dispatch_count() == 1 and short.workspace_requirement().size == 0
+    long = plan(4, 33)
+    assert long.dispatch_count() == 2 and long.workspace_requirement().alignment == 256
+    assert plan(1, 4096, window=300).dispatch_count() == 1  # a window of few tiles, whatever lies before it
+    assert plan(64, 4096).workspace_requirement().size < 64 << 20
+    assert hc.prepare(CTX, hc.PagedAttention(), D(BF16, [2, 8, 60]), D(BF16, [64, 2, 2, 16, 60]), D(I32, [2, 4096]), D(I32, [2])).dispatch_count() == 1

@@ -124,6 +124,42 @@ def test_batched_sequences(case):
     check_batched(operation, dtype, q, k, v, lengths, launch(operation, [q, k, v, *marks]))
 
 
+# as BATCHED, with enough tiles that a device is full of them: one wave to 32 rows instead of two
+MANY = [
+    ("bf16", 64, 8, 4, 40, 150, 150, None, True, 0, 0, True),
+    ("f16", 80, 8, 2, 40, 150, 170, None, True, 40, 3, True),
+    ("bf16", 128, 8, 2, 40, 150, 150, [150, 0, 129, 77] * 10, False, 0, 0, True),
+    ("f16", 256, 8, 2, 20, 150, 150, None, True, 0, 0, True),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=[f"{c[0]}-d{c[1]}-{c[4]}x{c[2]}" for c in MANY])
+def test_many_sequences(case):
+    test_batched_sequences(case)
+    want = "/128x2x32" if case[1] == 256 else "/128x1x64"
+    assert hc.last_launch_variant().endswith(want), hc.last_launch_variant()
+
+
+def test_the_shape_of_a_tile_follows_the_blocks():
+    rng = np.random.default_rng(8)
+    for depth, rows, want in ((64, 60, "d64/128x1x64"), (64, 200, "d64/128x2x64"), (96, 60, "d96/128x1x64"), (96, 200, "d96/128x2x64"),
+                              (128, 60, "d128/128x1x64"), (128, 200, "d128/128x2x64"), (256, 200, "d256/64x2x32")):
+        q, k, v = (values(rng, (rows, 2, depth), torch.bfloat16) for _ in range(3))
+        marks = torch.tensor([0, rows], dtype=torch.int32, device=DEVICE)
+        note(f"attention tiles of depth {depth}, {rows} rows")
+        operation = hc.Attention(depth ** -0.5)
+        check_packed(operation, torch.bfloat16, q, k, v, [0, rows], launch(operation, [q, k, v, marks]))
+        assert hc.last_launch_variant() == "attention_tiles/" + want
+
+
+def test_a_sequence_of_many_steps():
+    rng = np.random.default_rng(9)
+    q, k, v = values(rng, (1500, 2, 128), torch.bfloat16, 1.5), values(rng, (1500, 1, 128), torch.bfloat16), values(rng, (1500, 1, 128), torch.bfloat16)
+    note("attention of 1500 rows")
+    for operation in (hc.Attention(0.088, return_log_sum=True), hc.Attention(0.088, True, 333, 200, True), hc.Attention(0.088, False)):
+        check_packed(operation, torch.bfloat16, q, k, v, [0, 1500], launch(operation, [q, k, v]))
+
+
 @pytest.mark.parametrize("tag", ["bf16", "f16"])
 @pytest.mark.parametrize("depth", [64, 60])
 def test_heads_of_one_projection(tag, depth):

@@ -48,7 +48,7 @@ def narrowed(x, cache_type):
 
 APPENDS = [(tag, cache, depth, page, tokens)
            for tag, cache in (("bf16", "bf16"), ("f16", "f16"), ("f32", "f32"), ("bf16", "e4m3"), ("f16", "e4m3"), ("f32", "e4m3"))
-           for depth, page, tokens in ((128, 16, 1), (64, 1, 37), (80, 24, 700), (63, 7, 41), (256, 64, 130))]
+           for depth, page, tokens in ((128, 16, 1), (64, 1, 37), (80, 24, 700), (63, 7, 41), (256, 64, 130), (72, 16, 33))]
 
 
 @pytest.mark.parametrize("tag,cache_tag,depth,page,tokens", APPENDS)
@@ -212,6 +212,45 @@ def test_new_tokens_over_a_paged_cache(case):
     check(operation, query, paged, lengths, attend(operation, query, paged))
 
 
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("depth", [64, 48, 128, 80, 256, 144])
+@pytest.mark.parametrize("new,shared", [(1, 4), (3, 8), (8, 8)])
+def test_rows_of_a_key_head_and_depths(cache, depth, new, shared):
+    """16, 32 and 64 rows to a block, keys split and joined."""
+    rng, lengths = np.random.default_rng(depth + new), [700, 33, 0]
+    paged = Paged(rng, lengths, 2, depth, 16, TYPES[cache])
+    query = values(rng, (3, new, 2 * shared, depth), torch.bfloat16, 1.5)
+    note(f"paged attention {cache} depth {depth}, {new * shared} rows")
+    for operation in (hc.PagedAttention(depth ** -0.5, return_log_sum=True), hc.PagedAttention(depth ** -0.5, 100, 3, True)):
+        check(operation, query, paged, lengths, attend(operation, query, paged))
+        rows = 16 if new * shared <= 16 else 32 if new * shared <= 32 else 64
+        padded = 64 if depth <= 64 else 128 if depth <= 128 else 256
+        label = f"attention_split/{'e4m3/' if cache == 'e4m3' else ''}{'d' if depth == padded else 'below-d'}{padded}/{rows}-rows"
+        assert hc.last_launch_variant() == label + ("" if operation.window else f" + attention_join/d{padded}/row-to-block")
+
+
+@pytest.mark.parametrize("depth", [64, 128, 256])
+def test_many_rows_joined(depth):
+    rng, lengths = np.random.default_rng(depth), [1, 900] + [20, 0, 140] * 13
+    paged = Paged(rng, lengths, 4, depth, 16, torch.bfloat16)
+    query = values(rng, (len(lengths), 4, 16, depth), torch.bfloat16, 1.5)
+    operation = hc.PagedAttention(depth ** -0.5, return_log_sum=True)
+    note(f"paged attention of {len(lengths)} sequences of 64 rows, depth {depth}")
+    check(operation, query, paged, lengths, attend(operation, query, paged))
+    assert hc.last_launch_variant().endswith(f"attention_join/d{depth}/rows")
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (31, 0), (33, 1), (128, 130), (200, 31), (5000, 7)])
+def test_windows_at_every_offset(window, sinks):
+    """Windows that begin anywhere in a step, over sinks that end anywhere before them."""
+    rng, lengths = np.random.default_rng(window), list(range(1, 24, 3)) + list(range(150, 400, 23))
+    paged = Paged(rng, lengths, 1, 64, 16, torch.bfloat16)
+    query = values(rng, (len(lengths), 2, 2, 64), torch.bfloat16, 1.5)
+    operation = hc.PagedAttention(0.125, window, sinks, True)
+    note(f"paged attention windows {window} {sinks}")
+    check(operation, query, paged, lengths, attend(operation, query, paged))
+
+
 def test_many_sequences_of_every_length():
     rng = np.random.default_rng(21)
     lengths = [int(n) for n in rng.integers(0, 400, 150)] + [3000]
@@ -235,21 +274,38 @@ def test_free_slots_that_hold_no_numbers(tag, cache, depth, new):
 
 @pytest.mark.parametrize("tag", ["bf16", "f16"])
 @pytest.mark.parametrize("depth", [64, 128, 256])
-def test_new_tokens_do_not_see_those_behind_them(tag, depth):
+@pytest.mark.parametrize("queries", [2, 8, 16])
+def test_new_tokens_do_not_see_those_behind_them(tag, depth, queries):
     """The last new token's key and value are no numbers, and one key before the window of all but the first."""
     rng, lengths = np.random.default_rng(23), [100]
     paged = Paged(rng, lengths, 1, depth, 16, TYPES[tag])
     place = (int(paged.table[0, 99 // 16]), 99 % 16), (int(paged.table[0, 64 // 16]), 64 % 16)
     for page, at in place:
         paged.cache[page, 0, 0, at], paged.cache[page, 1, 0, at] = math.nan, math.inf
-    query = values(rng, (1, 4, 2, depth), TYPES[tag], 1.5)
+    query = values(rng, (1, 4, queries, depth), TYPES[tag], 1.5)
     operation = hc.PagedAttention(depth ** -0.5, 32)
-    note(f"paged attention of new tokens with NaN behind them {tag} {depth}")
+    note(f"paged attention of new tokens with NaN behind them {tag} {depth} {queries}")
     (out,) = attend(operation, query, paged)
     keys, vals = host(paged.keys[0]), host(paged.values[0])
     want, _, bound, _ = attention_rows(host(query[0]), keys, vals, 96, True, 32, 0, operation.scale, query.dtype)
     assert_within(out[0, :3], want[:3], bound[:3])  # queries 96..98 see keys from 65 on
     assert torch.isnan(out[0, 3]).all()
+
+
+@pytest.mark.parametrize("tag", ["bf16", "f16"])
+@pytest.mark.parametrize("queries", [2, 8, 16])
+def test_an_infinite_value_reaches_the_rows_that_see_it(tag, queries):
+    """Alone in a sequence's first key, among others, and in the newest of four tokens."""
+    rng, lengths = np.random.default_rng(28), [4, 60]
+    paged = Paged(rng, lengths, 1, 64, 16, TYPES[tag])
+    paged.cache[int(paged.table[0, 0]), 1, 0, 0, 5] = math.inf
+    paged.cache[int(paged.table[1, 3]), 1, 0, 58 % 16, 6] = -math.inf
+    query = values(rng, (2, 4, queries, 64), TYPES[tag])
+    note(f"paged attention of infinite values {tag} {queries}")
+    (out,) = attend(hc.PagedAttention(0.125), query, paged)
+    assert (out[0, :, :, 5] == math.inf).all() and (out[1, 2:, :, 6] == -math.inf).all()
+    out[0, :, :, 5], out[1, 2:, :, 6] = 0, 0
+    assert torch.isfinite(out).all()
 
 
 @pytest.mark.parametrize("tag,cache", [("bf16", "bf16"), ("f16", "e4m3"), ("f32", "f32")])
