@@ -2,14 +2,18 @@
 // keys and values of their type or e4m3, in memory or in a paged cache.
 //
 // Bound by the bytes of keys and values, which are read once for all rows of a key head (its query heads times the new
-// tokens).  The keys of all sequences, in tiles of 128, are dealt to about as many chunks as the device holds blocks, however
-// long each sequence is: a chunk is ceil(tiles / chunks) tiles of one sequence.  A block takes one chunk of one key head; its
-// four waves each take 32 keys of every tile and do not meet before the end:
-//   S^T[key, row] = K Q^T        (A: rows of K straight from memory, B: the queries)
-//   p = 2^(S^T c - m), O^T[dim, row] = V^T P^T   (A: columns of V by transposing reads of the wave's own LDS rows)
-// with the running maximum m and sum l of the softmax per lane (a lane's row is its column).  The next step's keys and values
-// are loaded while one is computed, the page numbers of the one after it too.  The waves' (m, l, O) are joined in LDS; a
-// sequence of one chunk is then done, others leave theirs in the workspace for the second kernel.
+// tokens).  The keys of all sequences, in tiles of 128, are dealt to a fixed number of chunks, however long each sequence is: a
+// chunk is ceil(tiles / chunks) tiles of one sequence.  A block takes one chunk of one key head:
+//   S^T[key, row] = K Q^T,  p = 2^(S^T c - m),  O^T[dim, row] = V^T P^T   (c = scale * log2(e))
+// with the running maximum m and sum l of the softmax per lane (a lane's row is its column).  Up to 16 rows, its four waves each
+// take 32 keys of every tile and do not meet before the end; 32 or 64 rows are dealt to the waves, which share the tile's keys
+// in LDS (64 rows to every wave spilled: 93 sequences of 8 new tokens, 8 key heads of 128, 118 us, shared 68).  Keys go through LDS
+// too, not only the values that are read by columns: whole rows side by side are whole cache lines, and only of those are
+// non-temporal loads fast (64 sequences of 30 to 16384 keys, 8 key heads of 128, bf16, 760 MB: 130 us, 5.8 TB/s of the 7.0 that a
+// large read reaches; loads of 64 bytes of a row 200, by plain loads 150; 16 of 20000 to 32768 in e4m3, 852 MB: 146 us, 5.85 TB/s).
+// The next tile's keys are asked for when this one's are in LDS, its values likewise, the page numbers of the one after it too.
+// The waves' (m, l, O) are joined in LDS; a sequence of one chunk is then done, others leave theirs in the workspace for the
+// second kernel.
 #include "attention_math.h"
 
 namespace hyle_hip {
@@ -49,7 +53,8 @@ __device__ __forceinline__ uint32_t scanned(uint32_t v, int lane) {
 }
 // The sequence and chunk that a slot of the grid is; false past the last.  Every wave of a launch comes to the same answer
 // from the marks alone.  target, chunks that all tiles are dealt to, is 0 where every sequence is one.  A block of one tile has
-// nothing to load while it computes, so a chunk has two at least where the tiles are more than the resident blocks.
+// nothing to load while it computes, so a chunk has two at least where the tiles are more than the resident blocks (one sequence
+// of 32751 keys, 2 key heads of 256: 24 us with chunks of two tiles, 34 with one, 26 with four).
 __device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t *marks, int slot, int target, int blocks, SplitChunk *c) {
   const int lane = (int)threadIdx.x % kWaveLanes;
   if (target == 0) {
@@ -71,7 +76,8 @@ __device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t
     const int index = base + lane;
     total += (uint32_t)__builtin_amdgcn_readlane((int)scanned(tiles_at(index, attention_mark(p, marks, min(index, p.sequences - 1))), lane), kWaveLanes - 1);
   }
-  const int each = (int)max((total + (uint32_t)target - 1) / (uint32_t)target, total > (uint32_t)blocks ? 2ull : 1ull);
+  // (never more than a sequence can have)
+  const int each = (int)min(max((total + (uint32_t)target - 1) / (uint32_t)target, total > (uint32_t)blocks ? 2ull : 1ull), 1ull << 24);
   int before = 0;
   for (int base = 0; base < p.sequences; base += kWaveLanes) {
     const int index = base + lane, mark = base == 0 ? first_mark : attention_mark(p, marks, min(index, p.sequences - 1));
@@ -552,7 +558,8 @@ constexpr int kUnsplit = 4;
 AttentionSplit attention_split_of(const AttentionParams &p, int compute_units) {
   AttentionSplit split;
   // The chunks of one key head and tile of rows: three rounds of the blocks that the device holds, so that the last ones of
-  // ragged sequences leave it idle for a third of a block.
+  // ragged sequences leave it idle for a third of a block (us with a half, one, two, three and four rounds: 64 ragged sequences 158,
+  // 140, 134, 130, 130; 16 long ones in e4m3 151, 178, 157, 146, 148).
   const int64_t lanes = (int64_t)p.heads * row_tiles_of(p);
   const int64_t blocks = (int64_t)compute_units * resident(p.narrow_cache, padded_depth(p), row_waves_of(p));
   const int64_t target = (3 * blocks + lanes - 1) / lanes;

@@ -1,7 +1,9 @@
 // paged_append.hip -- keys and values of new tokens to their slots of a paged cache [pages, 2, heads, page, depth].
 //
 // A thread moves eight elements of a head (16 bytes of f16 / bf16), sixteen for a cache of e4m3 where the depth allows, or, where
-// a row is not made of whole aligned vectors, one.  Bound by bytes: every element is read once and written once.
+// a row is not made of whole aligned vectors, one.  Bound by bytes: every element is read once and written once (8192 tokens of 8
+// heads of 128, bf16 to e4m3, 50 MB: 11.2 us, 4.5 TB/s where a large copy reaches 4.9; eight elements to a thread 14.1; 64 tokens
+// kept as bf16, 3.2 us, a launch).
 #include "attention.h"
 
 namespace hyle_hip {

@@ -1004,6 +1004,8 @@ hyle_hip_status admit_attention(hyle_hip_plan *p, uint32_t units) {
     a.v_row = value.byte_strides[row];
     a.v_head = value.byte_strides[row + 1];
     if (packed && a.sequences == 0) return HYLE_HIP_OK;  // every row is behind the last sequence
+    if ((uint64_t)a.sequences * (uint64_t)a.queries > kMaxElements / 2)
+      return fail(HYLE_HIP_UNIMPLEMENTED, "attention requires at most INT32_MAX / 2 heads of sequences");
   }
   a.shared = Divisor((uint32_t)(a.queries / a.heads));
   for (uint32_t i = 0; i < r.input_count; ++i) p->concat_input_bytes[i] = spanned_bytes(in[i]);

@@ -730,6 +730,10 @@ inline Result<PreparedOperation> prepare(const Context &c, const Operation &op, 
                                          const TensorDesc &b, const TensorDesc &d) noexcept {
   return prepare(c, op, {a, b, d});
 }
+inline Result<PreparedOperation> prepare(const Context &c, const Operation &op, const TensorDesc &a,
+                                         const TensorDesc &b, const TensorDesc &d, const TensorDesc &e) noexcept {
+  return prepare(c, op, {a, b, d, e});
+}
 
 }  // namespace compute
 }  // namespace hyle

@@ -221,6 +221,23 @@ HOST_TEST(GatherFollowsTheSchema) {
   EXPECT(trusted->dispatch_count() == 1 && trusted->workspace_requirement().size == 0);
 }
 
+HOST_TEST(AttentionAndItsCacheFollowTheSchema) {
+  const TensorDesc query = dense(DataType::kBFloat16, {2, 3, 8, 64}), keys = dense(DataType::kBFloat16, {2, 9, 4, 64});
+  auto out = infer_output_descriptions(Attention{.scale = 0.125F, .return_log_sum = true}, {query, keys, keys});
+  REQUIRE(out.has_value() && out->size() == 2);
+  EXPECT((*out)[0] == query && (*out)[1] == dense(DataType::kFloat32, {2, 3, 8}));
+  EXPECT(infer_output_descriptions(Attention{.causal = false, .window = 4}, {query, keys, keys}).error().IsInvalidArgument());
+  EXPECT(infer_output_descriptions(Attention{.sinks = 4}, {query, keys, keys}).error().IsInvalidArgument());
+  const TensorDesc cache = dense(DataType::kFloat8E4M3FN, {10, 2, 4, 16, 64});
+  out = infer_output_descriptions(PagedAttention{}, {query, cache, dense(DataType::kInt32, {2, 5}), dense(DataType::kInt32, {2})});
+  REQUIRE(out.has_value() && out->size() == 1);
+  EXPECT((*out)[0] == query);
+  out = infer_output_descriptions(PagedAppend{.pages = 10, .page_size = 16, .cache_type = DataType::kFloat8E4M3FN},
+                                  {dense(DataType::kBFloat16, {7, 4, 64}), dense(DataType::kBFloat16, {7, 4, 64}), dense(DataType::kInt32, {7})});
+  REQUIRE(out.has_value() && out->size() == 1);
+  EXPECT((*out)[0] == cache);
+}
+
 HOST_TEST(SubmitWithoutDeviceIsFailedPrecondition) {
   Context context = Context::planning_only();
   EXPECT(context.create_queue().error().IsFailedPrecondition());
@@ -713,6 +730,34 @@ DEVICE_TEST(RopeMatchesTheReferenceTestsKnownAnswers) {
   const float rates[2] = {0.5F, 0.25F};
   hyle_oracle_rope(HYLE_ORACLE_F32, values.data(), dims, 4, 1, steps, 0, 0, rates, 0, 4, 1, oracle.data());
   for (int i = 0; i < 16; ++i) EXPECT(std::fabs(got[i] - oracle[i]) <= 4e-6F * 24.0F);
+}
+
+DEVICE_TEST(PagedAttentionReadsWhatPagedAppendWrote) {
+  // two tokens of one head of four dims go to page 2 of a cache of three pages of two; a query at right angles to both keys
+  // weighs their values alike
+  const TensorDesc rows = dense(DataType::kFloat32, {2, 1, 4}), cache = dense(DataType::kFloat32, {3, 2, 1, 2, 4});
+  auto append = prepare(fixture().context, PagedAppend{.pages = 3, .page_size = 2, .cache_type = DataType::kFloat32}, rows, rows, dense(DataType::kInt32, {2}));
+  const TensorDesc query = dense(DataType::kFloat32, {1, 1, 4});
+  auto attend = prepare(fixture().context, PagedAttention{.scale = 0.5F}, query, cache, dense(DataType::kInt32, {1, 1}), dense(DataType::kInt32, {1}));
+  REQUIRE(append.has_value() && attend.has_value());
+  DeviceBuffer keys = upload(std::vector<float>{1, 0, 0, 0, 0, 1, 0, 0}), values = upload(std::vector<float>{1, 2, 3, 4, 3, 2, 1, 0});
+  DeviceBuffer slots = upload(std::vector<std::int32_t>{4, 5}), pages = upload(std::vector<std::int32_t>{2}), lengths = upload(std::vector<std::int32_t>{2});
+  DeviceBuffer held = upload(std::vector<float>(48, 7.0F)), q = upload(std::vector<float>{0, 0, 1, 1}), out = upload(std::vector<float>(4, 7.0F));
+  auto first = append->create_invocation();
+  auto second = attend->create_invocation();
+  REQUIRE(first.has_value() && second.has_value());
+  auto written = first->submit(fixture().queue, {*ConstTensorView::create(rows, keys), *ConstTensorView::create(rows, values),
+                                                 *ConstTensorView::create(dense(DataType::kInt32, {2}), slots)}, {*TensorView::create(cache, held)});
+  REQUIRE(written.has_value());
+  auto read = second->submit(fixture().queue, {*ConstTensorView::create(query, q), *ConstTensorView::create(cache, held),
+                                               *ConstTensorView::create(dense(DataType::kInt32, {1, 1}), pages),
+                                               *ConstTensorView::create(dense(DataType::kInt32, {1}), lengths)}, {*TensorView::create(query, out)});
+  REQUIRE(read.has_value());
+  EXPECT(read->wait().ok());
+  EXPECT(download<float>(out, 4) == std::vector<float>({2, 2, 2, 2}));
+  const std::vector<float> kept = download<float>(held, 48);
+  for (int i = 0; i < 32; ++i) EXPECT(kept[i] == 7.0F);
+  EXPECT(kept[32] == 1.0F && kept[37] == 1.0F && kept[40] == 1.0F && kept[44] == 3.0F);
 }
 
 DEVICE_TEST(RejectedSubmissionsEnqueueNothing) {
