@@ -1011,8 +1011,11 @@ hyle_hip_status admit_attention(hyle_hip_plan *p, uint32_t units) {
   for (uint32_t i = 0; i < r.input_count; ++i) p->concat_input_bytes[i] = spanned_bytes(in[i]);
   p->route = Route::kAttention;
   p->dispatches = 1;
-  // few rows to a key head leave the tiles of 128 rows empty and the device too, so the keys are split instead
-  p->attention_few_rows = paged || (!packed && (int64_t)a.rows * a.shared.divisor <= 64);
+  // Few rows to a key head leave the tiles of 128 rows empty and the device too, so the keys are split instead, where there are
+  // enough of them for the rows: more than a step of the tiles, or, for 64 rows, more than the split kernel leaves to one block (us,
+  // tiles / split, depth 128: 24 rows of 64 keys 6.6 / 7.6, of 100 7.9 / 7.5; 64 of 400 14.1 / 19.1, of 800 20.3 / 13.6).
+  const int64_t rows = (int64_t)a.rows * a.shared.divisor;
+  p->attention_few_rows = paged || (!packed && (rows <= 16 || (rows <= 32 && a.keys > 64) || (rows <= 64 && a.keys > 512)));
   if (p->attention_few_rows && attention_split_serves(p->elem, a, true)) {
     p->attention_split = attention_split_of(a, (int)units);
     p->workspace_size = p->attention_split.workspace;

@@ -152,6 +152,20 @@ def test_the_shape_of_a_tile_follows_the_blocks():
         assert hc.last_launch_variant() == "attention_tiles/" + want
 
 
+def test_few_rows_split_their_keys():
+    rng = np.random.default_rng(10)
+    for rows, shared, keys, want in ((1, 2, 3, "attention_split/d128/16-rows"), (16, 1, 300, "attention_split/d128/16-rows"),
+                                     (12, 2, 60, "attention_tiles/d128/128x1x64"), (12, 2, 300, "attention_split/d128/32-rows"),
+                                     (16, 4, 200, "attention_tiles/d128/128x2x64"), (16, 4, 1500, "attention_split/d128/64-rows + attention_join/d128/row-to-block")):
+        q, k, v = values(rng, (2, rows, 2 * shared, 128), torch.bfloat16, 1.5), values(rng, (2, keys, 2, 128), torch.bfloat16), values(rng, (2, keys, 2, 128), torch.bfloat16)
+        lengths = [keys, keys // 3]
+        marks = torch.tensor(lengths, dtype=torch.int32, device=DEVICE)
+        note(f"attention of {rows} x {shared} rows over {keys} keys")
+        for operation in (hc.Attention(0.088, return_log_sum=True), hc.Attention(0.088, False)):
+            check_batched(operation, torch.bfloat16, q, k, v, lengths, launch(operation, [q, k, v, marks]))
+            assert hc.last_launch_variant() == want, hc.last_launch_variant()
+
+
 def test_a_sequence_of_many_steps():
     rng = np.random.default_rng(9)
     q, k, v = values(rng, (1500, 2, 128), torch.bfloat16, 1.5), values(rng, (1500, 1, 128), torch.bfloat16), values(rng, (1500, 1, 128), torch.bfloat16)
