@@ -14,12 +14,19 @@ namespace {
 constexpr int kWaves = 8;
 constexpr int kMaxDepth = 256;
 constexpr int kDims = kMaxDepth / kWaveLanes;  // of a lane
+constexpr uint32_t kAcross = 1u << 22;  // blocks along x, whose threads are counted in 32 bits; further ones lie along y
+
+__host__ __device__ inline uint32_t blocks_of(const AttentionParams &p) {  // (no more than there are query elements)
+  return (uint32_t)p.rows * (p.kind == AttentionKind::kPacked ? 1u : (uint32_t)p.sequences) * (uint32_t)p.queries;
+}
 
 template <class T, class C>
 __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_rows(AttentionParams p, AttentionBuffers b) {
   __shared__ float query[kMaxDepth], weights[kWaves][kWaveLanes], joined[kWaves][kMaxDepth], tops[kWaves], sums[kWaves];
-  const int head = (int)(blockIdx.x % (uint32_t)p.queries);
-  int row = (int)(blockIdx.x / (uint32_t)p.queries), index;
+  const uint32_t block = blockIdx.y * kAcross + blockIdx.x;
+  if (block >= blocks_of(p)) return;
+  const int head = (int)(block % (uint32_t)p.queries);
+  int row = (int)(block / (uint32_t)p.queries), index;
   if (p.kind == AttentionKind::kPacked) {
     // the last sequence that begins at or before the row
     int low = 0, high = p.sequences - 1;
@@ -109,8 +116,9 @@ struct AttentionGeneralTag {
 };
 
 template <class T, class C> static void start(const AttentionParams &p, const AttentionBuffers &b, hipStream_t stream) {
-  const uint64_t rows = (uint64_t)p.rows * (p.kind == AttentionKind::kPacked ? 1u : (uint64_t)p.sequences);
-  hipLaunchKernelGGL((attention_rows<T, C>), dim3((uint32_t)(rows * (uint64_t)p.queries)), dim3(kWaves * kWaveLanes), 0, stream, p, b);
+  const uint32_t blocks = blocks_of(p);
+  const dim3 grid(blocks < kAcross ? blocks : kAcross, (blocks + kAcross - 1) / kAcross);
+  hipLaunchKernelGGL((attention_rows<T, C>), grid, dim3(kWaves * kWaveLanes), 0, stream, p, b);
 }
 
 hipError_t launch_attention_general(Elem type, const AttentionParams &p, const AttentionBuffers &b, hipStream_t stream) {

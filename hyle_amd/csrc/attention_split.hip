@@ -579,6 +579,9 @@ AttentionSplit attention_split_of(const AttentionParams &p, int compute_units) {
   split.slots = (int)slots;
   split.joined = most > kUnsplit && target > 1;
   if (!split.joined) split.target = 0, split.slots = p.sequences;
+  const uint64_t lines = (uint64_t)p.rows * p.shared.divisor * (uint64_t)p.heads * (uint64_t)p.sequences;
+  split.launches = axis_holds((uint64_t)split.slots * (uint64_t)lanes, kThreads) &&
+                   (!split.joined || axis_holds(lines * (uint64_t)(padded_depth(p) / 4) + join_threads(padded_depth(p), false), 1));
   const int64_t rows = (int64_t)p.rows * p.shared.divisor * p.heads * split.slots;
   split.stats_offset = ((size_t)rows * (size_t)p.depth * sizeof(float) + 255) / 256 * 256;
   split.places_offset = split.stats_offset + ((size_t)rows * sizeof(float2) + 255) / 256 * 256;

@@ -373,6 +373,8 @@ static void start(const AttentionParams &p, const AttentionBuffers &b, hipStream
 
 bool attention_tiles_serves(Elem type, const AttentionParams &p, bool vector_aligned) {
   if (type == Elem::kF32 || p.kind == AttentionKind::kPaged || !vector_aligned || p.depth % 8 != 0) return false;
+  // (so many blocks take the shapes of 128 rows, of depth 256 with two waves to each 32)
+  if (!axis_holds(slots_of(p, 128) * (uint64_t)p.queries, p.depth <= 128 ? 256 : 512)) return false;
   return ((p.q_sequence | p.q_row | p.q_head | p.k_sequence | p.k_row | p.k_head | p.v_sequence | p.v_row | p.v_head) % 16) == 0;
 }
 

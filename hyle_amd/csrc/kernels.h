@@ -376,6 +376,9 @@ struct Divisor {
   __host__ __device__ uint32_t quotient(uint32_t n) const { return (uint32_t)(((uint64_t)n * multiplier) >> shift); }
 };
 
+// An axis of a launch's grid counts threads in 32 bits.
+inline bool axis_holds(uint64_t blocks, uint64_t threads) { return blocks * threads <= 0xFFFFFFFFull; }
+
 // Attention of query rows over keys in memory or in a paged cache (hyle_hip.h has the rules).  Strides are in bytes.
 // marks: packed, the sequences' first rows and the end; else the valid keys of each sequence or null.
 enum class AttentionKind : uint8_t { kBatched, kPacked, kPaged };
@@ -403,10 +406,11 @@ struct AttentionBuffers {
   void *out = nullptr;
   float *logs = nullptr;
 };
-// The split over the keys: chunks that the keys are dealt to (0: one to a sequence), slots of the grid, whether a second kernel joins, the workspace.
+// The split over the keys: chunks that the keys are dealt to (0: one to a sequence), slots of the grid, whether a second kernel joins, whether grids hold
+// the blocks of both, the workspace.
 struct AttentionSplit {
   int target = 1, blocks = 1, slots = 0;
-  bool joined = false;
+  bool joined = false, launches = false;
   size_t stats_offset = 0, places_offset = 0, workspace = 0;
 };
 AttentionSplit attention_split_of(const AttentionParams &p, int compute_units);

@@ -1016,8 +1016,10 @@ hyle_hip_status admit_attention(hyle_hip_plan *p, uint32_t units) {
   // tiles / split, depth 128: 24 rows of 64 keys 6.6 / 7.6, of 100 7.9 / 7.5; 64 of 400 14.1 / 19.1, of 800 20.3 / 13.6).
   const int64_t rows = (int64_t)a.rows * a.shared.divisor;
   p->attention_few_rows = paged || (!packed && (rows <= 16 || (rows <= 32 && a.keys > 64) || (rows <= 64 && a.keys > 512)));
-  if (p->attention_few_rows && attention_split_serves(p->elem, a, true)) {
-    p->attention_split = attention_split_of(a, (int)units);
+  if (p->attention_few_rows && attention_split_serves(p->elem, a, true)) p->attention_split = attention_split_of(a, (int)units);
+  // (what no grid of the split kernel or of the tiles holds is attention_rows', whose grid has a second axis)
+  p->attention_few_rows = p->attention_few_rows && p->attention_split.launches;
+  if (p->attention_few_rows) {
     p->workspace_size = p->attention_split.workspace;
     p->workspace_alignment = p->workspace_size != 0 ? 256 : 1;
     p->dispatches = p->attention_split.joined ? 2 : 1;
