@@ -29,40 +29,34 @@ __device__ __forceinline__ float other_half_sum(float v) {
   return bits_f32(both[0]) + bits_f32(both[1]);
 }
 
-// Which tile of which sequence a slot of the grid is; false past the last.  Late tiles, which see the most keys, come first.
+// Which tile of which sequence a slot of the grid is; false where it is none.  Late tiles, which see the most keys, come first.
+// Packed sequence i, whose rows begin at b_i, has the places from first(i) = floor((b_i + (R - 1) i) / R) on: R rows to a tile,
+// first(i + 1) - first(i) is at least its ceil(rows / R) tiles, so places need no sum over the sequences before, and each block finds
+// its own by a search with 64 probes at a time (65536 sequences of one row, 8 heads: 3.3 ms, with a sum over all of them in each block 148; 7 or 64 sequences the same 8 us).
 __device__ __forceinline__ bool tile_of(const AttentionParams &p, const int32_t *marks, int slot, int rows_per_tile, int tiles, int *index, int *tile) {
   if (p.kind != AttentionKind::kPacked) {
     *tile = tiles - 1 - slot / p.sequences;
     *index = slot % p.sequences;
     return true;
   }
-  // packed: sequences have as many tiles as their rows fill; counted from the last one's last
   const int lane = (int)threadIdx.x % kWaveLanes;
-  int before = 0;
-  for (int last = p.sequences - 1; last >= 0; last -= kWaveLanes) {
-    const int mine = last - lane;
-    int count = 0;
-    if (mine >= 0) {
-      const AttentionSequence s = attention_sequence(p, marks, mine);
-      count = (s.rows + rows_per_tile - 1) / rows_per_tile;
-    }
-    int through = count;  // of this lane's sequence and those after it
-#pragma unroll
-    for (int step = 1; step < kWaveLanes; step *= 2) {
-      const int up = __shfl_up(through, step, kWaveLanes);
-      if (lane >= step) through += up;
-    }
-    const uint64_t holds = __ballot(slot < before + through);
-    if (holds != 0) {
-      const int at = __builtin_ctzll(holds);
-      const int end = before + __builtin_amdgcn_readlane(through, at);
-      *index = last - at;
-      *tile = end - 1 - slot;  // its last tile has the lowest slot
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(through, kWaveLanes - 1);
-  }
-  return false;
+  auto first = [&](int i, int begin) { return (int)(((uint64_t)begin + (uint64_t)(rows_per_tile - 1) * (uint64_t)i) / (uint32_t)rows_per_tile); };
+  const int place = first(p.sequences, p.rows) - 1 - slot;
+  int low = 0, count = p.sequences, step;  // the last sequence whose places begin at or before this one is among `count` from `low` on
+  do {
+    step = (count + kWaveLanes - 1) / kWaveLanes;
+    const int at = lane * step;
+    const bool before = at < count && first(low + at, min(max(marks[low + min(at, count - 1)], 0), p.rows)) <= place;
+    const uint64_t lanes = __ballot(before);
+    if (lanes == 0) return false;
+    const int last = (kWaveLanes - 1 - __builtin_clzll(lanes)) * step;
+    low += last;
+    count = min(step, count - last);
+  } while (step > 1);
+  const AttentionSequence s = attention_sequence(p, marks, low);
+  *index = low;
+  *tile = place - first(low, (int)s.row);
+  return *tile < (s.rows + rows_per_tile - 1) / rows_per_tile;
 }
 
 // Waves of a SIMD that the registers are kept for (one instead of two: 8192 tokens of 16 heads of 128 539 us instead of 311).

@@ -9,6 +9,7 @@ import torch
 from hyle_amd import compute as hc
 from hyle_amd import torch_io as tio
 
+from attention_support import assert_within, attention_rows
 from gpu_support import DEVICE, context, note
 
 pytestmark = pytest.mark.gpu
@@ -92,3 +93,48 @@ def test_a_paged_batch_past_a_grids_axis(batch):
     some = ~empty
     held = cache[table[some, 0].long()]
     assert_one_key(0.3, query[some][:, :, None], held[:, 0], held[:, 1], [out[some], logs[some]])
+
+
+@pytest.mark.parametrize("sequences", [64, 65, 4096, 4097, 70001, 2 ** 20 - 1])
+def test_packed_sequences_are_found_among_any_number_of_them(sequences):
+    """Sequences of no, one and, in places, some hundred rows: every tile finds its own."""
+    rng, queries = np.random.default_rng(sequences), 2 if sequences < 2 ** 17 else 16
+    lengths = rng.integers(0, 2, sequences)
+    for i, rows in ((0, 130), (sequences // 2, 300), (sequences - 1, 129)):
+        lengths[i] = rows
+    offsets = np.concatenate([[3], 3 + np.cumsum(lengths)]).astype(np.int32)
+    rows = int(offsets[-1]) + 5
+    q, k, v = (random(20 + i, (rows, heads, 8), torch.bfloat16) for i, heads in enumerate((queries, 1, 1)))
+    operation = hc.Attention(0.3, return_log_sum=True)
+    note(f"packed attention of {sequences} sequences")
+    outputs = launch(operation, [q, k, v, torch.from_numpy(offsets).to(DEVICE)])
+    assert hc.last_launch_variant().startswith("attention_tiles/d64/")
+    single = np.repeat(lengths, lengths) == 1
+    alone = torch.from_numpy(3 + np.flatnonzero(single)).to(DEVICE)
+    assert_one_key(0.3, q[alone][:, None], k[alone][:, None], v[alone][:, None], [t[alone] for t in outputs])
+    for i in (0, sequences // 2, sequences - 1):
+        span = slice(int(offsets[i]), int(offsets[i + 1]))
+        out, logs, bound, log_bound = attention_rows(*(t[span].double().cpu().numpy() for t in (q, k, v)), 0, True, 0, 0, 0.3, torch.bfloat16)
+        assert_within(outputs[0][span], out, bound)
+        assert_within(outputs[1][span], logs, log_bound)
+    for t in outputs:
+        assert (t[:3] == 77.0).all() and (t[-5:] == 77.0).all()
+
+
+def test_eight_times_the_sequences_take_about_eight_times_as_long():
+    """Not sixty-four times, as they do where every block looks through all sequences."""
+    def best(sequences):
+        q, k, v = (random(30 + i, (sequences, heads, 64), torch.bfloat16) for i, heads in enumerate((8, 2, 2)))
+        marks = torch.arange(sequences + 1, dtype=torch.int32, device=DEVICE)
+        bound = tio.Bound(context(), hc.Attention(0.125), [tio.desc_of(t) for t in (q, k, v, marks)])
+        outputs, times = bound.outputs(), []
+        for _ in range(6):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            bound.submit([q, k, v, marks], outputs)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+    note("packed attention of 4096 and of 32768 sequences")
+    assert best(2 ** 15) < 24 * best(2 ** 12)
