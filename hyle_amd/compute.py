@@ -542,7 +542,7 @@ class PagedAttention:
 class PagedAppend:
     """Inputs (keys, values [T, H, D], Int32 [T] slots): rows written to their slots (page * page_size + place) of the
     output, a cache [pages, 2, H, page_size, D] of `cache_type` (the keys' type or Float8E4M3FN), whose other rows stay
-    as they were.  A slot outside the cache writes nothing."""
+    as they were.  A slot outside the cache writes nothing; one that several tokens have ends with elements of any of them."""
     pages: int = 0
     page_size: int = 0
     cache_type: DataType = DataType.kUnknown

@@ -194,7 +194,8 @@ typedef enum hyle_hip_op_kind {
   /* Keys and values of new tokens into such a cache: in0 keys, in1 values [T, H, D] of one type, in2 I32 [T] slots
    * (page * page size + place in the page).  out0 is the cache, dense [P, 2, H, page, D]: `count` = P, `axis` = page
    * size, `kind` = its type (in0's or F8_E4M3FN: nearest even, beyond +-448 the nearest end, NaN stays).  Only the
-   * tokens' rows are written.  A slot outside the cache writes nothing; of two tokens with one slot either stays. */
+   * tokens' rows are written.  A slot outside the cache writes nothing.  Slots inside it should differ: one that
+   * several tokens have ends with elements of any of them, each as one of them has it at that place. */
   HYLE_HIP_OP_PAGED_APPEND = 0x107
 } hyle_hip_op_kind;
 
