@@ -616,8 +616,8 @@ def _op_desc(operation, inputs: Sequence[TensorDesc]) -> capi.OpDescC:
         c.op, c.kind = (OperationKind.kPagedAttention, 0) if paged else (OperationKind.kAttention, int(operation.causal))
         c.scale, c.count, c.axis, c.kind2 = operation.scale, operation.window, operation.sinks, int(operation.return_log_sum)
     elif isinstance(operation, PagedAppend):
-        if operation.pages < 0 or not 0 < operation.page_size <= _INT32_MAX:
-            raise StatusError(capi.INVALID_ARGUMENT, "PagedAppend requires a page count and a positive page size")
+        if not 0 <= operation.pages <= _INT32_MAX or not 0 < operation.page_size <= _INT32_MAX:
+            raise StatusError(capi.INVALID_ARGUMENT, "PagedAppend requires a page count and a positive page size within int32")
         c.op, c.kind, c.count, c.axis = OperationKind.kPagedAppend, int(operation.cache_type), operation.pages, operation.page_size
     else:
         raise StatusError(capi.UNIMPLEMENTED, f"operation {type(operation).__name__} is not served by this provider")

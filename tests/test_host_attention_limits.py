@@ -1,6 +1,8 @@
 """What attention plans ask for at the limits of a launch, without a device."""
 from __future__ import annotations
 
+import pytest
+
 from hyle_amd import compute as hc
 
 DT, D = hc.DataType, hc.TensorDesc.dense
@@ -15,3 +17,12 @@ def test_a_split_whose_blocks_no_grid_holds_is_not_planned():
     fits, past = plan(2 ** 22 - 2 ** 14), plan(2 ** 22)
     assert fits.dispatch_count() == 2 and fits.workspace_requirement().size > 0
     assert past.dispatch_count() == 1 and past.workspace_requirement().size == 0
+
+
+def test_more_pages_than_slots_can_count_are_refused():
+    """Also where the low 64 bits of the number are few."""
+    keys = D(BF16, [3, 4, 64])
+    for pages in (2 ** 31, 2 ** 64 + 10):
+        with pytest.raises(hc.StatusError) as refused:
+            hc.infer_output_descriptions(hc.PagedAppend(pages, 1, BF16), [keys, keys, D(I32, [3])])
+        assert refused.value.is_invalid_argument()
