@@ -47,7 +47,7 @@ __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_rows(AttentionP
   const AttentionSpan span = attention_span(p, s.keys, s.first + row);
   const unsigned char *q = attention_query(p, b, s, index, row, head);
   const int group = (int)p.shared.quotient((uint32_t)head), wave = (int)threadIdx.x / kWaveLanes, lane = (int)threadIdx.x % kWaveLanes;
-  for (int d = threadIdx.x; d < p.depth; d += kWaves * kWaveLanes) query[d] = Traits<T>::load(q, d) * p.scale;
+  for (int d = threadIdx.x; d < p.depth; d += kWaves * kWaveLanes) query[d] = Traits<T>::load(q, d);
   __syncthreads();
 
   float top = -INFINITY, sum = 0.0f, out[kDims] = {};
@@ -66,6 +66,7 @@ __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_rows(AttentionP
       const unsigned char *k = static_cast<const unsigned char *>(b.key) + place.key + (int64_t)group * p.k_head;
       score = 0.0f;
       for (int d = 0; d < p.depth; ++d) score = fmaf(query[d], Traits<C>::load(k, d), score);
+      score *= p.scale;  // (a query times the scale may pass f32's range where the product does not)
     }
     const float next = fmaxf(top, group_max<kWaveLanes>(score));
     const float shift = next == -INFINITY ? 0.0f : next;
