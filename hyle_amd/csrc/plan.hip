@@ -956,6 +956,7 @@ hyle_hip_status admit_attention(hyle_hip_plan *p, uint32_t units) {
   const int64_t depth = query.dims[query.rank - 1];
   if (depth > 256) return fail(HYLE_HIP_UNIMPLEMENTED, "attention serves depths up to 256");
   if (p->output_elements[0] > kMaxElements) return fail(HYLE_HIP_UNIMPLEMENTED, "attention requires at most INT32_MAX query elements");
+  if (std::fabs(r.scale) > 0x1p127f) return fail(HYLE_HIP_UNIMPLEMENTED, "attention serves scales up to 2^127");  // times log2(e) within f32
   if (p->output_elements[0] == 0) return HYLE_HIP_OK;
   AttentionParams &a = p->attention;
   const bool packed = !paged && query.rank == 3 && r.input_count == 4;

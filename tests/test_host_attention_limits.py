@@ -26,3 +26,14 @@ def test_more_pages_than_slots_can_count_are_refused():
         with pytest.raises(hc.StatusError) as refused:
             hc.infer_output_descriptions(hc.PagedAppend(pages, 1, BF16), [keys, keys, D(I32, [3])])
         assert refused.value.is_invalid_argument()
+
+
+def test_scales_whose_base_two_logarithms_pass_f32_are_declined():
+    q, cache = D(BF16, [2, 4, 64]), D(BF16, [8, 2, 4, 16, 64])
+    for scale in (2.0 ** 127, -2.0 ** 127):
+        assert hc.prepare(CTX, hc.Attention(scale), q, q, q).dispatch_count() == 1
+    for scale in (2.4e38, -3e38):
+        for operation, inputs in ((hc.Attention(scale), (q, q, q)), (hc.PagedAttention(scale), (q, cache, D(I32, [2, 3]), D(I32, [2])))):
+            with pytest.raises(hc.StatusError) as refused:
+                hc.prepare(CTX, operation, *inputs)
+            assert refused.value.code == hc.StatusCode.kUnimplemented
