@@ -572,7 +572,8 @@ AttentionSplit attention_split_of(const AttentionParams &p, int compute_units) {
   }
   split.target = (int)target;
   // The sum over the sequences of ceil(tiles / each), at least one for each of them, where each is at least total / target and,
-  // with more tiles than blocks, 2.
+  // with more tiles than blocks, 2.  (Sinks and a window that begins between two tiles can be one tile more than all keys, `most` + 1:
+  // half of that, rounded up, is within `most` / 2 and the sequence's own one.)
   int64_t slots = most * p.sequences / 2 > split.blocks ? most * p.sequences / 2 : split.blocks;
   if (target < slots) slots = target;
   slots += p.sequences;
