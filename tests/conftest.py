@@ -24,6 +24,19 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu)")
 
 
+# Modules whose cases reach launch shapes that no other module does, beside those that the coverage test itself asks for.
+COVERAGE_MODULES = ("test_gpu_attention", "test_gpu_paged_attention")
+
+
+def pytest_collection_modifyitems(items):
+    """The coverage test holds what a whole session launched; without all of the modules there is nothing to hold."""
+    collected = {item.module.__name__ for item in items if getattr(item, "module", None) is not None}
+    absent = [name for name in COVERAGE_MODULES if name not in collected]
+    for item in items:
+        if absent and getattr(item, "module", None) is not None and item.module.__name__ == "test_zy_launch_shape_coverage":
+            item.add_marker(pytest.mark.skip(reason=f"the whole GPU suite did not run in this session (not collected: {absent})"))
+
+
 def process_holds_gpu() -> bool:
     """True once this process has opened the GPU's compute device."""
     try:
