@@ -1014,9 +1014,14 @@ hyle_hip_status admit_attention(hyle_hip_plan *p, uint32_t units) {
   p->dispatches = 1;
   // Few rows to a key head leave the tiles of 128 rows empty and the device too, so the keys are split instead, where there are
   // enough of them for the rows: more than a step of the tiles, or, for 64 rows, more than the split kernel leaves to one block (us,
-  // tiles / split, depth 128: 24 rows of 64 keys 6.6 / 7.6, of 100 7.9 / 7.5; 64 of 400 14.1 / 19.1, of 800 20.3 / 13.6).
-  const int64_t rows = (int64_t)a.rows * a.shared.divisor;
-  p->attention_few_rows = paged || (!packed && (rows <= 16 || (rows <= 32 && a.keys > 64) || (rows <= 64 && a.keys > 512)));
+  // tiles / split, depth 128: 24 rows of 64 keys 6.6 / 7.6, of 100 7.9 / 7.5; 64 of 400 14.1 / 19.1, of 800 20.3 / 13.6).  Where query
+  // heads share keys and their tiles, one at least to a query head, are more than the compute units, these take turns over the same
+  // keys, and few keys are split too (64 rows of 512 keys, 4 query heads to a key head of depth 128: 256 tiles 15.1 / 18.3, 384 28.0 /
+  // 18.7, 8192 290 / 125; two to a key head: 320 tiles 28.2 / 20.0); of one step's keys two tiles run at once (64 keys, 512 tiles 8.0 / 9.8,
+  // 1024 13.8 / 12.1; of depth 256, 320 tiles 23.8 / 17.5).  Heads with keys of their own stay (1024 tiles of 512 keys 55.7 / 67.4).
+  const int64_t rows = (int64_t)a.rows * a.shared.divisor, tiles = (int64_t)a.sequences * a.queries;
+  const bool turns = a.shared.divisor > 1 && tiles > (a.keys <= 64 && depth <= 128 ? 2 : 1) * (int64_t)units;
+  p->attention_few_rows = paged || (!packed && (rows <= 16 || (rows <= 64 && (turns || a.keys > (rows <= 32 ? 64 : 512)))));
   if (p->attention_few_rows && attention_split_serves(p->elem, a, true)) p->attention_split = attention_split_of(a, (int)units);
   // (what no grid of the split kernel or of the tiles holds is attention_rows', whose grid has a second axis)
   p->attention_few_rows = p->attention_few_rows && p->attention_split.launches;
