@@ -5,7 +5,8 @@
 // tokens).  The keys of all sequences, in tiles of 128, are dealt to a fixed number of chunks, however long each sequence is: a
 // chunk is ceil(tiles / chunks) tiles of one sequence.  A block takes one chunk of one key head:
 //   S^T[key, row] = K Q^T,  p = 2^(S^T c - m),  O^T[dim, row] = V^T P^T   (c = scale * log2(e))
-// with the running maximum m and sum l of the softmax per lane (a lane's row is its column).  Up to 16 rows, its four waves each
+// with the running maximum m and sum l of the softmax per lane (a lane's row is its column).  Weights are rounded once to the
+// queries' type, which the matrix unit asks for; sums, statistics and what chunks leave are f32.  Up to 16 rows, its four waves each
 // take 32 keys of every tile and do not meet before the end; 32 or 64 rows are dealt to the waves, which share the tile's keys
 // in LDS (64 rows to every wave spilled: 93 sequences of 8 new tokens, 8 key heads of 128, 118 us, shared 68).  Keys go through LDS
 // too, not only the values that are read by columns: whole rows side by side are whole cache lines, and only of those are
@@ -552,7 +553,10 @@ int row_tiles_of(const AttentionParams &p) {
 }
 }  // namespace
 
-// Sequences of so few tiles are not split: a tile takes a block about 1 us, the second kernel 4.
+// Sequences of so few tiles are not split: a tile takes a block about 1 us, the second kernel 4.  (us, 512 keys unsplit / split, sequences
+// x key heads, depth 64: 4 x 8 7.7 / 8.7, 128 x 8 17.8 / 27.5; 128: 4 x 8 10.3 / 9.9, 32 x 8 11.7 / 14.9, 128 x 8 39.7 / 61; 256: 4 x 8 20.5 / 14.4,
+// 32 x 8 22.1 / 36.2, 128 x 8 95 / 105; 800 keys, depth 128: 4 x 8 15 / 10.9, 32 x 8 17.5 / 25.9.  So few sequences of depth 256 would
+// rather be split, and longer ones of a full device not.)
 constexpr int kUnsplit = 4;
 
 AttentionSplit attention_split_of(const AttentionParams &p, int compute_units) {
@@ -607,6 +611,9 @@ void start_split(const AttentionParams &p, const AttentionBuffers &b, const Spli
     hipLaunchKernelGGL((attention_split<T, C, kDepth, kRowWaves, false>), grid, block, 0, stream, p, b, layout);
   }
   if (!split.joined) return;
+  // Chunks side by side where rows are few (us of both kernels, side by side / a row to few threads, depth 64: 1024 rows of 16000 keys
+  // 31.1 / 48.3, 512 of 4000 26.1 / 28.8, 2048 of 4000 76.6 / 75.5, 4096 of 700 41.4 / 37.8; depth 256: 1024 of 16000 115 / 118, 2048 of 700
+  // 93 / 89, 4096 of 700 54.6 / 48.2).
   const uint32_t lines = layout.lines.divisor * (uint32_t)p.sequences;
   if (lines <= 2048) {
     note_variant<AttentionJoinTag<kDepth, true>>();

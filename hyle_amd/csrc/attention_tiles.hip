@@ -9,11 +9,15 @@
 // so the row statistics are per lane (a lane holds half of a query's keys, the lane 32 away the other half), and p feeds the
 // second product from the registers it was computed in: a lane's 8 keys of a 16-key step are 4h..4h+3 and 8+4h..8+4h+3 (h =
 // lane / 32), and the columns of V are read in that order too, for the sum over the keys does not care.
-// Weights are rounded once to the values' type, which the matrix unit asks for; sums and statistics are f32.
-// Bound by the matrix and the vector units, which a wave uses in turn: 8192 causal tokens of 16 heads of 128, bf16, take 307 to
-// 352 us by the machine (780 to 897 TFLOP/s of the 1190 of a large matrix product), the matrix unit is busy for 38 % of the cycles,
-// the vector unit for 46 % (a quarter-rate power to each weight is 512 of its 1250 cycles of a wave's step, the products are 1024),
-// LDS for 29 %, with no bank conflict.  Steps of 32 keys with three waves a SIMD took 359 where this took 307.
+// Weights are rounded once to the values' type, which the matrix unit asks for; sums and statistics, those that the rounded weights'
+// products are divided by too, are f32.  (Outputs in bf16 are off by 0.0021 of their size in root mean square, rounded from f32
+// throughout by 0.0016; f16 0.00028 and 0.0002.)
+// Bound by the matrix and the vector units, which a wave uses in turn: 8192 causal tokens of 16 heads of 128, bf16, take 304 to
+// 352 us by the machine (780 to 905 TFLOP/s of the 1190 of a large matrix product), the matrix unit is busy for 38 % of the cycles,
+// the vector unit for 44 % (a quarter-rate power to each weight is 512 of its 1250 cycles of a wave's step, the products are 1024),
+// LDS for 30 %, with no bank conflict; the rest is not accounted for.  Steps of 32 keys with three waves a SIMD took 359 where this took
+// 307.  Depth 256 is bound by registers: two waves a SIMD spill 45 of them, queries that are read back between the products of every step
+// (4096 tokens of 16 heads 277 us, 500 TFLOP/s), one wave a SIMD moves its outputs between the two halves of the register file.
 // O is rescaled only when a maximum has grown by more than kSlack (2^8 stays exact in every type here).
 #include "attention_math.h"
 
@@ -377,8 +381,9 @@ hipError_t launch_attention_tiles(Elem type, const AttentionParams &p, const Att
   // the loads' latency (us, one wave / two: 1500 tokens of 32 heads, depth 128, 384 blocks 52.1 / 39.2; 3000 of 16, 384 blocks
   // 96.1 / 70.2; 2000 of 32, depth 64, 512 blocks 46.7 / 39.0; 5000 of 16, 640 blocks 171 / 169; 8 padded sequences of 12 heads,
   // depth 64, 672 blocks 33.0 / 44.7; 8192 of 16, 1024 blocks 308 / 335).  One step of keys has no halves (16 tokens 7.3 / 8.2).
-  // At depth 256 two waves always, of 64 rows up to a block to a compute unit (2048 tokens of 16 heads, 128 rows 133, 64 rows
-  // 115; 4096 of 16, 281 / 400; with a window of 300, 4 heads, 43.7 / 30.4).
+  // At depth 256 two waves always, of 64 rows (one wave a SIMD, nothing spilled) up to a block to a compute unit, then of 128 (two
+  // waves, 45 registers spilled) (2048 tokens of 16 heads, 128 rows 133, 64 rows 112; 4096 of 16, 277 / 400; with a window of 300,
+  // 4 heads, 43.7 / 30.4).
   const uint64_t blocks = slots_of(p, 128) * (uint64_t)p.queries;
   auto typed = [&](auto tag) {
     using T = decltype(tag);

@@ -189,7 +189,8 @@ typedef enum hyle_hip_op_kind {
    * whose elements are the values themselves), in2 I32 [B, M] pages of each sequence in order, in3 I32 [B] lengths:
    * the keys of each sequence, the new tokens' own among them (keys past M * page do not exist).  Query i stands at
    * position in3 - R + i.  A page outside [0, P) holds no keys and is never read.  `scale`, `count`, `axis` and
-   * `kind2` as for ATTENTION; always causal.  A contiguous cache is one page per sequence. */
+   * `kind2` as for ATTENTION; always causal.  A contiguous cache is one page per sequence.  Made for a few new
+   * tokens: of R in the hundreds, every 64 rows of a key head read all keys that any row of their sequence sees. */
   HYLE_HIP_OP_PAGED_ATTENTION = 0x106,
   /* Keys and values of new tokens into such a cache: in0 keys, in1 values [T, H, D] of one type, in2 I32 [T] slots
    * (page * page size + place in the page).  out0 is the cache, dense [P, 2, H, page, D]: `count` = P, `axis` = page
