@@ -229,6 +229,9 @@ class OperationKind(enum.IntEnum):
     kAttention = 0x105
     kPagedAttention = 0x106
     kPagedAppend = 0x107
+    kRotaryAppend = 0x108
+    kPageBounds = 0x109
+    kPagedSelect = 0x10A
 
 
 class UnaryKind(enum.IntEnum):
@@ -530,8 +533,9 @@ class Attention:
 @dataclass(frozen=True)
 class PagedAttention:
     """The newest tokens of each sequence against a paged cache.  Inputs (queries [B, R, Hq, D] or [B, Hq, D], cache
-    [P, 2, H, page, D] of their type or Float8E4M3FN, pages Int32 [B, M], lengths Int32 [B] that count the new tokens).
-    Query i stands at position length - R + i; a page outside [0, P) holds no keys.  Outputs as Attention's."""
+    [P, 2, H, page, D] of their type or Float8E4M3FN, or of 4 bits, UInt8 [P, 2, H, page, 17 D / 32], pages Int32 [B, M],
+    lengths Int32 [B] that count the new tokens).  Query i stands at position length - R + i; a page outside [0, P) holds no
+    keys.  Pages [B, H, M] with lengths [B, H] are those of each key head (PagedSelect).  Outputs as Attention's."""
     scale: float = 1.0
     window: int = 0
     sinks: int = 0
@@ -541,11 +545,41 @@ class PagedAttention:
 @dataclass(frozen=True)
 class PagedAppend:
     """Inputs (keys, values [T, H, D], Int32 [T] slots): rows written to their slots (page * page_size + place) of the
-    output, a cache [pages, 2, H, page_size, D] of `cache_type` (the keys' type or Float8E4M3FN), whose other rows stay
-    as they were.  A slot outside the cache writes nothing; one that several tokens have ends with elements of any of them."""
+    output, a cache [pages, 2, H, page_size, D] of `cache_type` (the keys' type or Float8E4M3FN; UInt8: 4 bits, [..,
+    17 D / 32], codes of a page's rows and then a scale to 32 of their elements), whose other rows stay as they were.  A slot
+    outside the cache writes nothing; one that several tokens have ends with elements of any of them."""
     pages: int = 0
     page_size: int = 0
     cache_type: DataType = DataType.kUnknown
+
+
+@dataclass(frozen=True)
+class RotaryAppend:
+    """RoPE and PagedAppend in one.  Inputs (projected rows [T, Hq + 2 key_heads, D]: queries, keys, values; Int32 / Int64
+    [T] positions, F32 frequencies [rotary / 2] or [T, rotary / 2], Int32 [T] slots).  Outputs: the cache, as PagedAppend's,
+    and, with query heads, the rotated queries [T, Hq, D]."""
+    pages: int = 0
+    page_size: int = 0
+    cache_type: DataType = DataType.kUnknown
+    key_heads: int = 0
+    layout: RopeLayout = RopeLayout.kInterleaved
+
+
+@dataclass(frozen=True)
+class PageBounds:
+    """Inputs (cache, pages Int32 [B, M], lengths Int32 [B]): the least and largest key of every channel, BFloat16 [P, 2, H, D],
+    of the pages that hold each sequence's `newest` last tokens (0: all its pages).  Other pages' bounds stay as they were."""
+    newest: int = 0
+
+
+@dataclass(frozen=True)
+class PagedSelect:
+    """Inputs (queries [B, R, Hq, D] or [B, Hq, D], BFloat16 bounds [P, 2, H, D], pages Int32 [B, M], lengths Int32 [B]): for
+    every key head the first page, those of the newest tokens and, up to `count`, those in which the queries' products can be
+    largest.  Outputs: pages Int32 [B, H, count] in their order, -1 behind them, and their keys Int32 [B, H]: what PagedAttention
+    takes."""
+    count: int = 0
+    page_size: int = 0
 
 
 def _op_desc(operation, inputs: Sequence[TensorDesc]) -> capi.OpDescC:
@@ -619,6 +653,19 @@ def _op_desc(operation, inputs: Sequence[TensorDesc]) -> capi.OpDescC:
         if not 0 <= operation.pages <= _INT32_MAX or not 0 < operation.page_size <= _INT32_MAX:
             raise StatusError(capi.INVALID_ARGUMENT, "PagedAppend requires a page count and a positive page size within int32")
         c.op, c.kind, c.count, c.axis = OperationKind.kPagedAppend, int(operation.cache_type), operation.pages, operation.page_size
+    elif isinstance(operation, RotaryAppend):
+        if not 0 <= operation.pages <= _INT32_MAX or not 0 < operation.page_size <= _INT32_MAX or not 0 < operation.key_heads <= _INT32_MAX:
+            raise StatusError(capi.INVALID_ARGUMENT, "RotaryAppend requires a page count, a positive page size and key heads within int32")
+        c.op, c.kind, c.count, c.axis = OperationKind.kRotaryAppend, int(operation.cache_type), operation.pages, operation.page_size
+        c.kind2, c.axes_count, c.axes[0] = int(operation.layout), 1, operation.key_heads
+    elif isinstance(operation, PageBounds):
+        if not 0 <= operation.newest <= _INT32_MAX:
+            raise StatusError(capi.INVALID_ARGUMENT, "PageBounds requires a number of newest tokens within int32")
+        c.op, c.count = OperationKind.kPageBounds, operation.newest
+    elif isinstance(operation, PagedSelect):
+        if not 0 <= operation.count <= _INT32_MAX or not 0 < operation.page_size <= _INT32_MAX:
+            raise StatusError(capi.INVALID_ARGUMENT, "PagedSelect requires a count and a positive page size within int32")
+        c.op, c.count, c.axis = OperationKind.kPagedSelect, operation.count, operation.page_size
     else:
         raise StatusError(capi.UNIMPLEMENTED, f"operation {type(operation).__name__} is not served by this provider")
     if len(inputs) > capi.MAX_INPUTS:

@@ -1,23 +1,15 @@
-// attention.h -- what the attention kernels share: which rows and keys a sequence has, where a key stands, which keys a
-// query sees, and the decoder of e4m3 caches.
+// attention.h -- what the attention kernels share: which rows and keys a sequence has, where a key stands and which keys a
+// query sees.
 #pragma once
 
-#include "device_common.h"
-#include "kernels.h"
+#include "cache_types.h"
 
 namespace hyle_hip {
 
-struct E4M3 {};
-template <> struct Traits<E4M3> {
-  static constexpr int kSize = 1;
-  static __device__ __forceinline__ float load(const void *p, size_t i) {
-    return __builtin_amdgcn_cvt_f32_fp8((int)static_cast<const uint8_t *>(p)[i], 0);
-  }
-};
-
-// One sequence of a launch.  `first` is the position of its first query; its queries are rows `row` on of the output.
+// One sequence of a launch.  `first` is the position of its first query; its queries are rows `row` on of the output, of row `batch`
+// of the batch.  `head` is added to the launch's key heads (a sequence that is one key head of its row).
 struct AttentionSequence {
-  int rows, keys, first;
+  int rows, keys, first, batch, head;
   int64_t row;
 };
 
@@ -31,7 +23,9 @@ __device__ __forceinline__ AttentionSequence attention_sequence_of(const Attenti
   s.rows = p.rows;
   s.keys = min(mark, p.keys);
   s.first = (p.kind == AttentionKind::kPaged ? mark : p.keys) - p.rows;
-  s.row = (int64_t)index * p.rows;
+  s.batch = (int)p.apart.quotient((uint32_t)index);
+  s.head = index - s.batch * (int)p.apart.divisor;
+  s.row = (int64_t)s.batch * p.rows;
   return s;
 }
 __device__ __forceinline__ AttentionSequence attention_sequence(const AttentionParams &p, const int32_t *marks, int index) {
@@ -39,7 +33,8 @@ __device__ __forceinline__ AttentionSequence attention_sequence(const AttentionP
   AttentionSequence s;
   const int begin = min(max(marks[index], 0), p.rows), end = min(max(marks[index + 1], begin), p.rows);
   s.rows = s.keys = end - begin;
-  s.first = 0;
+  s.first = s.head = 0;
+  s.batch = index;
   s.row = begin;
   return s;
 }
@@ -61,14 +56,14 @@ __device__ __forceinline__ bool attention_sees(const AttentionParams &p, const A
 }
 
 __device__ __forceinline__ const unsigned char *attention_query(const AttentionParams &p, const AttentionBuffers &b, const AttentionSequence &s,
-                                                                int index, int row, int head) {
-  const int64_t at = p.kind == AttentionKind::kPacked ? (s.row + row) * p.q_row : (int64_t)index * p.q_sequence + (int64_t)row * p.q_row;
+                                                                int row, int head) {
+  const int64_t at = p.kind == AttentionKind::kPacked ? (s.row + row) * p.q_row : (int64_t)s.batch * p.q_sequence + (int64_t)row * p.q_row;
   return static_cast<const unsigned char *>(b.query) + at + (int64_t)head * p.q_head;
 }
 
 // Byte offsets of key `key` of head 0 from the operands' first bytes; false where a paged key has no page in the cache.
 struct AttentionPlace {
-  int64_t key, value;
+  int64_t key, value, scale;  // scale: of a cache in 4 bits, of keys and values alike
 };
 __device__ __forceinline__ bool attention_place(const AttentionParams &p, const int32_t *table, const AttentionSequence &s, int index, int key,
                                                 AttentionPlace *place) {
@@ -76,8 +71,10 @@ __device__ __forceinline__ bool attention_place(const AttentionParams &p, const 
     const uint32_t column = p.page.quotient((uint32_t)key), at = (uint32_t)key - column * p.page.divisor;
     const int32_t page = table[(int64_t)index * p.table_row + column];
     place->key = place->value = (int64_t)page * p.k_sequence + (int64_t)at * p.k_row;
+    place->scale = (int64_t)page * p.k_sequence + p.scale_offset + (int64_t)at * (p.k_row / 16);
     return (uint32_t)page < (uint32_t)p.pages;
   }
+  place->scale = 0;
   const int64_t row = p.kind == AttentionKind::kPacked ? s.row + key : key;
   const int64_t sequence = p.kind == AttentionKind::kPacked ? 0 : index;
   place->key = sequence * p.k_sequence + row * p.k_row;

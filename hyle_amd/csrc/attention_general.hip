@@ -17,7 +17,13 @@ constexpr int kDims = kMaxDepth / kWaveLanes;  // of a lane
 constexpr uint32_t kAcross = 1u << 22;  // blocks along x, whose threads are counted in 32 bits; further ones lie along y
 
 __host__ __device__ inline uint32_t blocks_of(const AttentionParams &p) {  // (no more than there are query elements)
-  return (uint32_t)p.rows * (p.kind == AttentionKind::kPacked ? 1u : (uint32_t)p.sequences) * (uint32_t)p.queries;
+  return (uint32_t)p.rows * (p.kind == AttentionKind::kPacked ? 1u : (uint32_t)p.sequences / p.apart.divisor) * (uint32_t)p.queries;
+}
+
+// Element d of a key or value at its codes' address; `scales`, of a cache in 4 bits.
+template <class C> __device__ __forceinline__ float element(const unsigned char *at, const unsigned char *scales, int d) {
+  if constexpr (std::is_same<C, MX4>::value) return mx4_element(at, scales, d);
+  else return Traits<C>::load(at, d);
 }
 
 template <class T, class C>
@@ -43,10 +49,12 @@ __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_rows(AttentionP
     index = row / p.rows;
     row -= index * p.rows;
   }
+  const int group = (int)p.shared.quotient((uint32_t)head);
+  if (p.apart.divisor != 1) index = index * (int)p.apart.divisor + group;  // a sequence of its own
   const AttentionSequence s = attention_sequence(p, b.marks, index);
   const AttentionSpan span = attention_span(p, s.keys, s.first + row);
-  const unsigned char *q = attention_query(p, b, s, index, row, head);
-  const int group = (int)p.shared.quotient((uint32_t)head), wave = (int)threadIdx.x / kWaveLanes, lane = (int)threadIdx.x % kWaveLanes;
+  const unsigned char *q = attention_query(p, b, s, row, head);
+  const int wave = (int)threadIdx.x / kWaveLanes, lane = (int)threadIdx.x % kWaveLanes;
   for (int d = threadIdx.x; d < p.depth; d += kWaves * kWaveLanes) query[d] = Traits<T>::load(q, d);
   __syncthreads();
 
@@ -58,14 +66,15 @@ __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_rows(AttentionP
   for (int g = wave; g < groups; g += kWaves) {
     const int first = g < before ? g * kWaveLanes : low + (g - before) * kWaveLanes;
     const int end = g < before ? sinks : span.high;
-    AttentionPlace place{0, 0};
+    AttentionPlace place{0, 0, 0};
     bool seen = first + lane < end;
     if (seen) seen = attention_place(p, b.table, s, index, first + lane, &place);
     float score = -INFINITY;
     if (seen) {
       const unsigned char *k = static_cast<const unsigned char *>(b.key) + place.key + (int64_t)group * p.k_head;
+      const unsigned char *k_scales = static_cast<const unsigned char *>(b.key) + place.scale + (int64_t)group * p.k_head;
       score = 0.0f;
-      for (int d = 0; d < p.depth; ++d) score = fmaf(query[d], Traits<C>::load(k, d), score);
+      for (int d = 0; d < p.depth; ++d) score = fmaf(query[d], element<C>(k, k_scales, d), score);
       score *= p.scale;  // (a query times the scale may pass f32's range where the product does not)
     }
     const float next = fmaxf(top, group_max<kWaveLanes>(score));
@@ -84,11 +93,16 @@ __global__ __launch_bounds__(kWaves * kWaveLanes) void attention_rows(AttentionP
       const float w = weights[wave][j];
       const int64_t at = ((int64_t)__builtin_amdgcn_readlane((int)(place.value >> 32), j) << 32) |
                          (uint32_t)__builtin_amdgcn_readlane((int)place.value, j);
-      const unsigned char *v = static_cast<const unsigned char *>(b.value) + at + (int64_t)group * p.v_head;
+      const unsigned char *v = static_cast<const unsigned char *>(b.value) + at + (int64_t)group * p.v_head, *v_scales = v;
+      if constexpr (std::is_same<C, MX4>::value) {
+        const int64_t scale_at = ((int64_t)__builtin_amdgcn_readlane((int)(place.scale >> 32), j) << 32) |
+                                 (uint32_t)__builtin_amdgcn_readlane((int)place.scale, j);
+        v_scales = static_cast<const unsigned char *>(b.value) + scale_at + (int64_t)group * p.v_head;
+      }
 #pragma unroll
       for (int i = 0; i < kDims; ++i) {
         const int d = lane + i * kWaveLanes;
-        if (d < p.depth) out[i] = fmaf(w, Traits<C>::load(v, d), out[i]);
+        if (d < p.depth) out[i] = fmaf(w, element<C>(v, v_scales, d), out[i]);
       }
     }
   }
@@ -125,9 +139,9 @@ template <class T, class C> static void start(const AttentionParams &p, const At
 hipError_t launch_attention_general(Elem type, const AttentionParams &p, const AttentionBuffers &b, hipStream_t stream) {
   note_variant<AttentionGeneralTag>();
   switch (type) {
-    case Elem::kF32: p.narrow_cache ? start<F32, E4M3>(p, b, stream) : start<F32, F32>(p, b, stream); break;
-    case Elem::kF16: p.narrow_cache ? start<F16, E4M3>(p, b, stream) : start<F16, F16>(p, b, stream); break;
-    case Elem::kBF16: p.narrow_cache ? start<BF16, E4M3>(p, b, stream) : start<BF16, BF16>(p, b, stream); break;
+    case Elem::kF32: p.four_bits ? start<F32, MX4>(p, b, stream) : p.narrow_cache ? start<F32, E4M3>(p, b, stream) : start<F32, F32>(p, b, stream); break;
+    case Elem::kF16: p.four_bits ? start<F16, MX4>(p, b, stream) : p.narrow_cache ? start<F16, E4M3>(p, b, stream) : start<F16, F16>(p, b, stream); break;
+    case Elem::kBF16: p.four_bits ? start<BF16, MX4>(p, b, stream) : p.narrow_cache ? start<BF16, E4M3>(p, b, stream) : start<BF16, BF16>(p, b, stream); break;
   }
   return hipGetLastError();
 }

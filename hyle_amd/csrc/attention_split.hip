@@ -124,6 +124,22 @@ template <class T> __device__ __forceinline__ void widened(u32x4 w, u32x4 *low, 
   *low = u32x4{a.x, a.y, b.x, b.y};
   *high = u32x4{c.x, c.y, d.x, d.y};
 }
+// 32 values in 4 bits as sixteen words of T by their scale: exact, but for f16's range.
+template <class T> __device__ __forceinline__ u32x4 widened4(uint32_t w, float scale) {
+  u32x4 out;
+  if constexpr (std::is_same<T, BF16>::value) {
+    out.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+    out.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
+    out.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
+    out.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+  } else {
+    out.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0));
+    out.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1));
+    out.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2));
+    out.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3));
+  }
+  return out;
+}
 __device__ __forceinline__ float rows_max(float v) {  // over the lanes of one column: 16 apart
   const auto a = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
   v = fmaxf(bits_f32(a[0]), bits_f32(a[1]));
@@ -155,10 +171,10 @@ constexpr int resident(bool narrow, int depth, int row_waves) {
   return depth <= 64 ? 4 : depth <= 128 ? (narrow ? 3 : 2) : narrow ? 2 : 1;
 }
 template <class T, class C, int kDepth, int kRowWaves, bool kWhole>
-__global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kDepth, kRowWaves)) void attention_split(AttentionParams p, AttentionBuffers b, SplitLayout layout) {
-  constexpr bool kNarrow = std::is_same<C, E4M3>::value;
+__global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDepth, kRowWaves)) void attention_split(AttentionParams p, AttentionBuffers b, SplitLayout layout) {
+  constexpr bool kNarrow = std::is_same<C, E4M3>::value, kFour = std::is_same<C, MX4>::value;
   constexpr int kSteps = kDepth / 32, kDims = kDepth / 16;
-  constexpr int kLoad = kNarrow ? 16 : 8;                // elements of a 16-byte vector
+  constexpr int kLoad = kFour ? 32 : kNarrow ? 16 : 8;   // elements of a 16-byte vector
   constexpr int kVectors = kDepth / kLoad;               // of a row
   constexpr int kLoads = kStep * kVectors / kWaveLanes;  // of a lane, for a step's keys or values
   constexpr int kRow = kDepth * 2 + 32;                  // bytes of a row in LDS: 8 rows of 32 bytes fill the banks
@@ -195,8 +211,8 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
 #pragma unroll
   for (int d = 0; d < kDims; ++d) out[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const unsigned char *keys = static_cast<const unsigned char *>(b.key) + (int64_t)group * p.k_head;
-  const unsigned char *values = static_cast<const unsigned char *>(b.value) + (int64_t)group * p.v_head;
+  const unsigned char *keys = static_cast<const unsigned char *>(b.key) + (int64_t)(group + s.head) * p.k_head;
+  const unsigned char *values = static_cast<const unsigned char *>(b.value) + (int64_t)(group + s.head) * p.v_head;
   const bool paged = p.kind == AttentionKind::kPaged;
   const int32_t *table = paged ? b.table + (int64_t)chunk.index * p.table_row : nullptr;
   auto first_of = [&](int tile) { return tile < tiles.sinks ? tile * kTile : tiles.low + (tile - tiles.sinks) * kTile; };
@@ -208,17 +224,28 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
   // One step's keys and values, whole rows side by side: a load's 64 vectors are whole cache lines, which non-temporal loads
   // need.  The next keys are asked for once these are in LDS, and so are the values.
   u32x4 key_words[kLoads], value_words[kLoads];
+  uint32_t key_scales[kFour ? kLoads : 1], value_scales[kFour ? kLoads : 1];  // bytes
   uint32_t alive = 0;  // bit j: key j of the step is there and some row sees it
   int64_t value_at = 0;
+  int scales_at = 0;  // from the codes of a row to its scales
   const int vectors = p.depth / kLoad;  // of a row; zeros past them
   const int vector = lane % kVectors;
-  auto fetch = [&](const unsigned char *from, int64_t place, u32x4 (&words)[kLoads]) {
+  auto fetch = [&](const unsigned char *from, int64_t place, u32x4 (&words)[kLoads], uint32_t *scales) {
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
       const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
       const int64_t at = ((int64_t)__shfl((int)(place >> 32), row, kWaveLanes) << 32) | (uint32_t)__shfl((int)place, row, kWaveLanes);
       if (!kWhole) words[k] = u32x4{0, 0, 0, 0};
-      if (kWhole || vector < vectors) words[k] = load16_stream(from + at, vector);
+      if constexpr (kFour) {
+        const int there = __shfl(scales_at, row, kWaveLanes);
+        if (!kWhole) scales[k] = 0;
+        if (kWhole || vector < vectors) {
+          words[k] = load16_words(from + at, vector);
+          scales[k] = from[at + there + vector];
+        }
+      } else {
+        if (kWhole || vector < vectors) words[k] = load16_stream(from + at, vector);
+      }
     }
   };
   auto fetch_keys = [&](int tile, int page) {
@@ -230,22 +257,31 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
       const uint32_t at = (uint32_t)known - p.page.quotient((uint32_t)known) * p.page.divisor;
       // (a page that is not there is read as the cache's first row, which is there: its keys are not alive)
       key_at = value_at = there ? (int64_t)page * p.k_sequence + (int64_t)at * p.k_row : 0;
+      if constexpr (kFour) scales_at = (int)p.scale_offset - (there ? (int)at * ((int)p.k_row / 16 * 15) : 0);
     } else {
       key_at = (int64_t)chunk.index * p.k_sequence + (int64_t)known * p.k_row;
       value_at = (int64_t)chunk.index * p.v_sequence + (int64_t)known * p.v_row;
     }
     alive = (uint32_t)__ballot(there);
-    fetch(keys, key_at, key_words);
+    fetch(keys, key_at, key_words, key_scales);
   };
-  auto fetch_values = [&]() { fetch(values, value_at, value_words); };
-  // a step's vectors to the wave's rows in LDS, e4m3 as the elements of T that they stand for
-  auto put = [&](unsigned char *base, const u32x4 (&words)[kLoads]) {
+  auto fetch_values = [&]() { fetch(values, value_at, value_words, value_scales); };
+  // a step's vectors to the wave's rows in LDS, e4m3 and 4 bits as the elements of T that they stand for (kClean: numbers alone)
+  auto put = [&](unsigned char *base, const u32x4 (&words)[kLoads], const uint32_t *scales, auto clean) {
+    constexpr bool kClean = decltype(clean)::value;
     __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses are in order)
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
       const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
       unsigned char *to = base + row * kRow + vector * kLoad * 2;
-      if constexpr (kNarrow) {
+      if constexpr (kFour) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          u32x4 wide = widened4<T>(words[k][w], bits_f32(scales[k] << 23));
+          if (kClean) wide = numbers_only<T>(wide);
+          *reinterpret_cast<u32x4 *>(to + 16 * w) = wide;
+        }
+      } else if constexpr (kNarrow) {
         u32x4 low, high;
         widened<T>(words[k], &low, &high);
         *reinterpret_cast<u32x4 *>(to) = low;
@@ -266,7 +302,7 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
   AttentionSpan span;
   {
     const int row = first_row + 16 * row_wave + column, known = min(row, layout.rows - 1), token = (int)p.shared.quotient((uint32_t)known);
-    const unsigned char *from = attention_query(p, b, s, chunk.index, token, group * (int)p.shared.divisor + known - token * (int)p.shared.divisor);
+    const unsigned char *from = attention_query(p, b, s, token, (group + s.head) * (int)p.shared.divisor + known - token * (int)p.shared.divisor);
     span = attention_span(p, s.keys, s.first + token);
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
@@ -293,7 +329,10 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
       const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
-      if (((these >> row) & 1u) == 0) value_words[k] = u32x4{0, 0, 0, 0};
+      if (((these >> row) & 1u) == 0) {
+        value_words[k] = u32x4{0, 0, 0, 0};
+        if constexpr (kFour) value_scales[k] = 0;
+      }
     }
   };
   // Values that are no numbers, of keys that not every row sees: a weight of 0 would make NaN of them in the product.  They are
@@ -319,17 +358,25 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
   auto any_no_number = [&]() {
     uint32_t found = 0;
 #pragma unroll
-    for (int k = 0; k < kLoads; ++k) found |= no_numbers<C>(value_words[k]);
+    for (int k = 0; k < kLoads; ++k) {
+      // (of 4 bits by the scale: from which on 6 of it, or 4, may pass T's range, and NaN)
+      if constexpr (kFour) found |= (uint32_t)(value_scales[k] >= (std::is_same<T, BF16>::value ? 253u : 141u));
+      else found |= no_numbers<C>(value_words[k]);
+    }
     return __ballot(found != 0) != 0;
   };
-  auto keep_numbers = [&]() {
+  auto keep_numbers = [&]() {  // (4 bits are cleaned on the way to LDS)
+    if constexpr (!kFour) {
 #pragma unroll
-    for (int k = 0; k < kLoads; ++k) value_words[k] = numbers_only<C>(value_words[k]);
+      for (int k = 0; k < kLoads; ++k) value_words[k] = numbers_only<C>(value_words[k]);
+    }
   };
+  constexpr std::false_type kAsRead{};
+  constexpr std::true_type kNumbers{};
 
   for (int tile = begin; tile < end; ++tile) {
     const uint32_t own = alive;
-    put(key_rows(wave), key_words);
+    put(key_rows(wave), key_words, key_scales, kAsRead);
     if constexpr (kRowWaves == 1) {
       __builtin_amdgcn_sched_barrier(0);  // (loads that move up further need registers of their own)
       if (tile + 1 < end) {
@@ -341,7 +388,7 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
       if (lane == 0) shared_alive[wave] = own;
       const bool odd = s.rows > 1 && !(own == 0xFFFFFFFFu && seen_whole(first_key(tile))) && any_no_number();
       if (odd && lane == 0) no_number = tile + 1;
-      put(value_rows(wave), value_words);
+      put(value_rows(wave), value_words, value_scales, kAsRead);
       __syncthreads();
       if (no_number == tile + 1) {
 #pragma unroll 1
@@ -351,7 +398,7 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
         }
         __syncthreads();
         keep_numbers();
-        put(value_rows(wave), value_words);
+        put(value_rows(wave), value_words, value_scales, kNumbers);
         __syncthreads();
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -412,12 +459,14 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
       }
       if constexpr (kRowWaves == 1) {
         clear_dead(these);
-        if (!whole && s.rows > 1 && any_no_number()) {
-          put(value_rows(wave), value_words);
+        const bool odd = !whole && s.rows > 1 && any_no_number();
+        if (odd) {
+          put(value_rows(wave), value_words, value_scales, kAsRead);
           add_no_numbers(value_rows(wave), these, first);
           keep_numbers();
         }
-        put(value_rows(wave), value_words);
+        if (kFour && odd) put(value_rows(wave), value_words, value_scales, kNumbers);
+        else put(value_rows(wave), value_words, value_scales, kAsRead);
         __builtin_amdgcn_sched_barrier(0);
         if (tile + 1 < end) fetch_values();
       }
@@ -456,7 +505,7 @@ __global__ __launch_bounds__(kThreads, resident(std::is_same<C, E4M3>::value, kD
     all += joined_sum[g * kRowWaves + join_wave][join_column] * keep[g];
   }
   const int token = (int)p.shared.quotient((uint32_t)row);
-  const int64_t at = (s.row + token) * p.queries + group * (int)p.shared.divisor + row - token * (int)p.shared.divisor;
+  const int64_t at = (s.row + token) * p.queries + (group + s.head) * (int)p.shared.divisor + row - token * (int)p.shared.divisor;
   const int64_t part = ((int64_t)slot * p.heads + group) * layout.rows + row;
   const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
   for (int d = (int)threadIdx.x % kRowThreads * 4; d < p.depth; d += kRowThreads * 4) {
@@ -519,7 +568,8 @@ __global__ __launch_bounds__(join_threads(kDepth, kSide)) void attention_join(At
     for (int i = 1; i < kParts; ++i) out += joined[i][dim / 4], sum += sums[i];
   }
   const int group = rest / layout.rows, row = rest - group * layout.rows, token = (int)p.shared.quotient((uint32_t)row);
-  const int64_t at = ((int64_t)index * p.rows + token) * p.queries + group * (int)p.shared.divisor + row - token * (int)p.shared.divisor;
+  const int batch = (int)p.apart.quotient((uint32_t)index), head = group + index - batch * (int)p.apart.divisor;
+  const int64_t at = ((int64_t)batch * p.rows + token) * p.queries + head * (int)p.shared.divisor + row - token * (int)p.shared.divisor;
   if (has) {
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
     uint2 w;
@@ -534,7 +584,7 @@ __global__ __launch_bounds__(join_threads(kDepth, kSide)) void attention_join(At
 
 template <class C, int kDepth, int kRowWaves, bool kWhole> struct AttentionSplitTag {
   static std::string text() {
-    return std::string("attention_split/") + (std::is_same<C, E4M3>::value ? "e4m3/" : "") + (kWhole ? "d" : "below-d") + std::to_string(kDepth) + "/" + std::to_string(16 * kRowWaves) + "-rows";
+    return std::string("attention_split/") + (std::is_same<C, E4M3>::value ? "e4m3/" : std::is_same<C, MX4>::value ? "mx4/" : "") + (kWhole ? "d" : "below-d") + std::to_string(kDepth) + "/" + std::to_string(16 * kRowWaves) + "-rows";
   }
 };
 template <int kDepth, bool kSide> struct AttentionJoinTag {
@@ -565,7 +615,7 @@ AttentionSplit attention_split_of(const AttentionParams &p, int compute_units) {
   // ragged sequences leave it idle for a third of a block (us with a half, one, two, three and four rounds: 64 ragged sequences 158,
   // 140, 134, 130, 130; 16 long ones in e4m3 151, 178, 157, 146, 148).
   const int64_t lanes = (int64_t)p.heads * row_tiles_of(p);
-  const int64_t blocks = (int64_t)compute_units * resident(p.narrow_cache, padded_depth(p), row_waves_of(p));
+  const int64_t blocks = (int64_t)compute_units * resident(p.narrow_cache || p.four_bits, padded_depth(p), row_waves_of(p));
   const int64_t target = (3 * blocks + lanes - 1) / lanes;
   split.blocks = (int)((blocks + lanes - 1) / lanes);
   // tiles of a sequence: of all its keys, or of the window of its new tokens and the sinks
@@ -594,8 +644,10 @@ AttentionSplit attention_split_of(const AttentionParams &p, int compute_units) {
   return split;
 }
 
+// (vectors of codes are read at addresses of whole words)
 bool attention_split_serves(Elem type, const AttentionParams &p, bool vector_aligned) {
-  if (type == Elem::kF32 || p.kind == AttentionKind::kPacked || !vector_aligned || p.depth % (p.narrow_cache ? 16 : 8) != 0) return false;
+  if (type == Elem::kF32 || p.kind == AttentionKind::kPacked || !vector_aligned || p.depth % (p.four_bits ? 32 : p.narrow_cache ? 16 : 8) != 0) return false;
+  if (p.four_bits) return ((p.q_sequence | p.q_row | p.q_head) % 16 | (p.k_sequence | p.k_head | p.value_offset) % 4) == 0 && p.scale_offset <= INT32_MAX / 2;
   return ((p.q_sequence | p.q_row | p.q_head | p.k_sequence | p.k_row | p.k_head | p.v_sequence | p.v_row | p.v_head) % 16) == 0;
 }
 
@@ -655,10 +707,12 @@ hipError_t launch_attention_split(Elem type, const AttentionParams &p, const Att
   layout.stats = reinterpret_cast<float2 *>(static_cast<unsigned char *>(workspace) + split.stats_offset);
   layout.places = reinterpret_cast<int2 *>(static_cast<unsigned char *>(workspace) + split.places_offset);
   if (type == Elem::kF16) {
-    if (p.narrow_cache) split_by_depth<F16, E4M3>(p, b, layout, split, stream);
+    if (p.four_bits) split_by_depth<F16, MX4>(p, b, layout, split, stream);
+    else if (p.narrow_cache) split_by_depth<F16, E4M3>(p, b, layout, split, stream);
     else split_by_depth<F16, F16>(p, b, layout, split, stream);
   } else {
-    if (p.narrow_cache) split_by_depth<BF16, E4M3>(p, b, layout, split, stream);
+    if (p.four_bits) split_by_depth<BF16, MX4>(p, b, layout, split, stream);
+    else if (p.narrow_cache) split_by_depth<BF16, E4M3>(p, b, layout, split, stream);
     else split_by_depth<BF16, BF16>(p, b, layout, split, stream);
   }
   return hipGetLastError();

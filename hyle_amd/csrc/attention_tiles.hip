@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyWaves * kWaveLanes, resident(kDepth
   const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
   {
     const int row = wave_row + column;
-    const unsigned char *from = attention_query(p, b, s, index, min(row, s.rows - 1), head);
+    const unsigned char *from = attention_query(p, b, s, min(row, s.rows - 1), head);
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       const int chunk = 2 * k + half;

@@ -18,6 +18,7 @@ constexpr int kWaveLanes = 64;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_element __attribute__((ext_vector_type(4), aligned(2)));  // at any element's address
+typedef uint32_t u32x4_words __attribute__((ext_vector_type(4), aligned(4)));    // at any word's
 
 struct F32 {};
 struct F16 {};
@@ -151,6 +152,9 @@ __device__ __forceinline__ void loads_issued(uint32_t &a) { asm volatile("" : "+
 // carry the non-temporal hint; small reused operands use the plain forms.
 __device__ __forceinline__ u32x4 load16_stream(const void *base, size_t vec) {
   return __builtin_nontemporal_load(static_cast<const u32x4 *>(base) + vec);
+}
+__device__ __forceinline__ u32x4 load16_words(const void *base, size_t vec) {  // streaming, at an address of whole words
+  return __builtin_nontemporal_load(static_cast<const u32x4_words *>(base) + vec);
 }
 __device__ __forceinline__ u32x4 load16(const void *base, size_t vec) {
   return static_cast<const u32x4 *>(base)[vec];

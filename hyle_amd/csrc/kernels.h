@@ -385,7 +385,9 @@ enum class AttentionKind : uint8_t { kBatched, kPacked, kPaged };
 struct AttentionParams {
   AttentionKind kind = AttentionKind::kBatched;
   bool causal = true, narrow_cache = false;  // narrow: keys and values in e4m3
-  int32_t sequences = 0;
+  bool four_bits = false;                    // keys and values in 4 bits: k_row is that of the codes, scale_offset from a head's codes to its scales
+  int32_t sequences = 0;                     // paged with a table of every key head: each of them is a sequence, and `heads` is 1
+  Divisor apart;                             // sequences to a row of the batch: key heads with tables of their own, else 1
   int32_t rows = 0;   // of each sequence; packed: of all
   int32_t keys = 0;   // most keys of a sequence
   int32_t queries = 0, heads = 0, depth = 0;  // query heads, key heads
@@ -396,6 +398,7 @@ struct AttentionParams {
   int64_t k_sequence = 0, k_row = 0, k_head = 0;  // paged: k_sequence is the page's
   int64_t v_sequence = 0, v_row = 0, v_head = 0;
   int64_t value_offset = 0;                       // paged: from the keys to the values
+  int64_t scale_offset = 0;
   int32_t pages = 0, columns = 0;
   int64_t table_row = 0;  // entries
   Divisor page;
@@ -421,14 +424,52 @@ bool attention_tiles_serves(Elem type, const AttentionParams &p, bool vector_ali
 hipError_t launch_attention_tiles(Elem type, const AttentionParams &p, const AttentionBuffers &b, int compute_units, hipStream_t stream);
 hipError_t launch_attention_general(Elem type, const AttentionParams &p, const AttentionBuffers &b, hipStream_t stream);
 
+// What a cache keeps an element in: the type of the tokens, e4m3, or 4 bits with a scale to 32 elements (cache_types.h).
+enum class CacheKind : uint8_t { kKept, kNarrow, kFourBits };
+
 // PagedAppend: rows of [tokens, heads, depth] keys and values to their slots of a dense cache.
 struct AppendParams {
   uint32_t tokens = 0, heads = 0, depth = 0, pages = 0;
-  bool narrow_cache = false;
+  CacheKind cache = CacheKind::kKept;
   int64_t k_token = 0, k_head = 0, v_token = 0, v_head = 0;  // bytes
   Divisor page;
 };
 hipError_t launch_paged_append(Elem type, const AppendParams &p, const void *keys, const void *values, const int32_t *slots,
                                void *cache, bool vector_aligned, hipStream_t stream);
+
+// RotaryAppend: projected rows [tokens, queries + 2 heads, depth], the queries and keys rotated on the way to `rotated` [tokens, queries,
+// depth] and the cache.  Frequencies are f32 [rotary / 2] or, stepped, [tokens, rotary / 2].
+struct RotaryAppendParams {
+  uint32_t tokens = 0, queries = 0, heads = 0, depth = 0, rotary = 0, pages = 0;
+  bool half_split = false, wide_positions = false, stepped_frequencies = false;
+  CacheKind cache = CacheKind::kKept;
+  int64_t token = 0, head = 0;  // bytes
+  Divisor page;
+};
+hipError_t launch_rotary_append(Elem type, const RotaryAppendParams &p, const void *projected, const void *positions, const void *frequencies,
+                                const int32_t *slots, void *cache, void *rotated, bool vector_aligned, hipStream_t stream);
+
+// PageBounds: the least and largest key of every channel of the pages that hold each sequence's newest tokens (0: any), outward to bf16.
+struct PageBoundsParams {
+  Elem type = Elem::kBF16;
+  CacheKind cache = CacheKind::kKept;
+  uint32_t sequences = 0, columns = 0, heads = 0, depth = 0, pages = 0;
+  uint32_t newest = 0, span = 0;  // span: columns that a sequence's newest tokens can lie in
+  int64_t page_bytes = 0, head_bytes = 0, row_bytes = 0, scale_offset = 0, table_row = 0;
+  Divisor page;
+};
+hipError_t launch_page_bounds(const PageBoundsParams &p, const void *cache, const int32_t *table, const int32_t *lengths, void *bounds,
+                              bool vector_aligned, hipStream_t stream);
+
+// PagedSelect: scores of pages [sequences, heads, columns] (f32, the workspace), then the best `count` of each key head in order.
+struct PagedSelectParams {
+  uint32_t sequences = 0, rows = 0, columns = 0, heads = 0, queries = 0, depth = 0, pages = 0, count = 0;
+  int64_t q_sequence = 0, q_row = 0, q_head = 0;        // bytes
+  int64_t b_page = 0, b_side = 0, b_head = 0, table_row = 0;  // the bounds' bytes; entries of the table
+  Divisor page, shared;
+};
+hipError_t launch_paged_select(Elem type, const PagedSelectParams &p, const void *query, const void *bounds, const int32_t *table,
+                               const int32_t *lengths, int32_t *selected, int32_t *seen, void *workspace, bool vector_aligned,
+                               hipStream_t stream);
 
 }  // namespace hyle_hip

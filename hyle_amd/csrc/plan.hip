@@ -284,6 +284,23 @@ hyle_hip_status expect_gguf_weight(const Desc &w) {
   return HYLE_HIP_OK;
 }
 
+// Elements of a cache's rows: of 4 bits, 32 to 17 bytes.  -1 where its bytes are no whole blocks.
+int64_t cached_depth(const Desc &cache) {
+  if (cache.dtype != HYLE_HIP_DTYPE_U8) return cache.dims[4];
+  return cache.dims[4] % 17 == 0 ? cache.dims[4] / 17 * 32 : -1;
+}
+// The cache [pages, 2, heads, page, depth] that an append writes.
+hyle_hip_status infer_cache(const hyle_hip_op_desc &r, const char *what, uint8_t type, int64_t heads, int64_t depth, Desc *out) {
+  if (r.kind != type && r.kind != HYLE_HIP_DTYPE_F8_E4M3FN && r.kind != HYLE_HIP_DTYPE_U8)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "%s requires a cache of the tokens' type, float8 e4m3 or 4 bits (uint8)", what);
+  if (r.kind == HYLE_HIP_DTYPE_U8 && depth % 32 != 0)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "%s requires a depth of whole blocks of 32 for a cache of 4 bits", what);
+  if (r.axis <= 0 || r.count > (uint64_t)std::numeric_limits<int32_t>::max() / (uint64_t)r.axis)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "%s requires a positive page size and slots within int32", what);
+  const int64_t dims[5] = {(int64_t)r.count, 2, heads, r.axis, r.kind == HYLE_HIP_DTYPE_U8 ? depth / 32 * 17 : depth};
+  return make_dense((uint8_t)r.kind, dims, 5, out);
+}
+
 // Attention and PagedAttention (hyle_hip.h has the operands' shapes)
 hyle_hip_status infer_attention(const hyle_hip_op_desc &r, Desc *outs, uint32_t *out_count) {
   const bool paged = r.op == HYLE_HIP_OP_PAGED_ATTENTION;
@@ -297,13 +314,16 @@ hyle_hip_status infer_attention(const hyle_hip_op_desc &r, Desc *outs, uint32_t 
   int64_t heads;
   if (paged) {
     const Desc &cache = in[1], &table = in[2], &lengths = in[3];
-    if (cache.rank != 5 || cache.dims[1] != 2 || cache.dims[4] != depth)
+    if (cache.rank != 5 || cache.dims[1] != 2 || cached_depth(cache) != depth)
       return fail(HYLE_HIP_INVALID_ARGUMENT, "paged attention requires a cache [pages, 2, heads, page, depth] of the queries' depth");
-    if (cache.dtype != query.dtype && cache.dtype != HYLE_HIP_DTYPE_F8_E4M3FN)
-      return fail(HYLE_HIP_INVALID_ARGUMENT, "paged attention requires a cache of the queries' type or float8 e4m3");
-    if (table.dtype != HYLE_HIP_DTYPE_I32 || table.rank != 2 || lengths.dtype != HYLE_HIP_DTYPE_I32 || lengths.rank != 1 ||
-        table.dims[0] != query.dims[0] || lengths.dims[0] != query.dims[0])
-      return fail(HYLE_HIP_INVALID_ARGUMENT, "paged attention requires i32 pages [sequences, columns] and i32 lengths [sequences]");
+    if (cache.dtype != query.dtype && cache.dtype != HYLE_HIP_DTYPE_F8_E4M3FN && cache.dtype != HYLE_HIP_DTYPE_U8)
+      return fail(HYLE_HIP_INVALID_ARGUMENT, "paged attention requires a cache of the queries' type, float8 e4m3 or 4 bits (uint8)");
+    const int axes = table.rank == 3 ? 2 : 1;  // of the table and the lengths: sequences, and key heads with pages of their own
+    if (table.dtype != HYLE_HIP_DTYPE_I32 || table.rank != axes + 1 || lengths.dtype != HYLE_HIP_DTYPE_I32 || lengths.rank != axes ||
+        table.dims[0] != query.dims[0] || lengths.dims[0] != query.dims[0] ||
+        (axes == 2 && (table.dims[1] != cache.dims[2] || lengths.dims[1] != cache.dims[2])))
+      return fail(HYLE_HIP_INVALID_ARGUMENT, "paged attention requires i32 pages [sequences, columns] and i32 lengths [sequences], or both with "
+                                             "an axis of the key heads behind the sequences'");
     heads = cache.dims[2];
   } else {
     const int rank = query.rank;
@@ -349,12 +369,76 @@ hyle_hip_status infer_paged_append(const hyle_hip_op_desc &r, Desc *outs) {
     return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedAppend requires floating keys and values [tokens, heads, depth] of one type and shape");
   if (slots.dtype != HYLE_HIP_DTYPE_I32 || slots.rank != 1 || slots.dims[0] != keys.dims[0])
     return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedAppend requires i32 slots [tokens]");
-  if (r.kind != keys.dtype && r.kind != HYLE_HIP_DTYPE_F8_E4M3FN)
-    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedAppend requires a cache of the keys' type or float8 e4m3");
-  if (r.axis <= 0 || r.count > (uint64_t)std::numeric_limits<int32_t>::max() / (uint64_t)r.axis)
-    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedAppend requires a positive page size and slots within int32");
-  const int64_t dims[5] = {(int64_t)r.count, 2, keys.dims[1], r.axis, keys.dims[2]};
-  return make_dense((uint8_t)r.kind, dims, 5, &outs[0]);
+  return infer_cache(r, "PagedAppend", keys.dtype, keys.dims[1], keys.dims[2], &outs[0]);
+}
+
+hyle_hip_status infer_rotary_append(const hyle_hip_op_desc &r, Desc *outs, uint32_t *out_count) {
+  const Desc *in = r.inputs;
+  hyle_hip_status s;
+  if ((s = expect_inputs(r, 4, 4)) != HYLE_HIP_OK) return s;
+  const Desc &rows = in[0], &positions = in[1], &frequencies = in[2], &slots = in[3];
+  if (!is_floating(rows.dtype) || rows.rank != 3)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "RotaryAppend requires floating rows [tokens, query heads + 2 key heads, depth]");
+  if (r.axes_count != 1 || r.axes[0] <= 0 || rows.dims[1] < 2 * (int64_t)r.axes[0])
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "RotaryAppend requires a positive number of key heads, twice which the rows hold");
+  if (!is_index(positions.dtype) || positions.rank != 1 || positions.dims[0] != rows.dims[0])
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "RotaryAppend requires i32 or i64 positions [tokens]");
+  const int64_t pairs = frequencies.rank > 0 ? frequencies.dims[frequencies.rank - 1] : 0;
+  if (frequencies.dtype != HYLE_HIP_DTYPE_F32 || frequencies.rank < 1 || frequencies.rank > 2 ||
+      (frequencies.rank == 2 && frequencies.dims[0] != rows.dims[0]) || pairs < 1 || pairs > rows.dims[2] / 2)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "RotaryAppend requires f32 frequencies [rotary / 2] or [tokens, rotary / 2] within the depth");
+  if (slots.dtype != HYLE_HIP_DTYPE_I32 || slots.rank != 1 || slots.dims[0] != rows.dims[0])
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "RotaryAppend requires i32 slots [tokens]");
+  if (r.kind2 > HYLE_HIP_ROPE_HALF_SPLIT) return fail(HYLE_HIP_INVALID_ARGUMENT, "RotaryAppend layout is invalid");
+  if ((s = infer_cache(r, "RotaryAppend", rows.dtype, r.axes[0], rows.dims[2], &outs[0])) != HYLE_HIP_OK) return s;
+  const int64_t dims[3] = {rows.dims[0], rows.dims[1] - 2 * (int64_t)r.axes[0], rows.dims[2]};
+  if (dims[1] == 0) return HYLE_HIP_OK;
+  *out_count = 2;
+  return make_dense(rows.dtype, dims, 3, &outs[1]);
+}
+
+hyle_hip_status infer_page_bounds(const hyle_hip_op_desc &r, Desc *outs) {
+  const Desc *in = r.inputs;
+  hyle_hip_status s;
+  if ((s = expect_inputs(r, 3, 3)) != HYLE_HIP_OK) return s;
+  const Desc &cache = in[0], &table = in[1], &lengths = in[2];
+  if ((!is_floating(cache.dtype) && cache.dtype != HYLE_HIP_DTYPE_U8) || cache.rank != 5 || cache.dims[1] != 2 || cached_depth(cache) < 0)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PageBounds requires a cache [pages, 2, heads, page, depth], floating or of 4 bits (uint8)");
+  if (table.dtype != HYLE_HIP_DTYPE_I32 || table.rank != 2 || lengths.dtype != HYLE_HIP_DTYPE_I32 || lengths.rank != 1 ||
+      table.dims[0] != lengths.dims[0])
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PageBounds requires i32 pages [sequences, columns] and i32 lengths [sequences]");
+  if (r.count > (uint64_t)std::numeric_limits<int32_t>::max())
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PageBounds requires a number of newest tokens within int32");
+  const int64_t dims[4] = {cache.dims[0], 2, cache.dims[2], cached_depth(cache)};
+  return make_dense(HYLE_HIP_DTYPE_BF16, dims, 4, &outs[0]);
+}
+
+hyle_hip_status infer_paged_select(const hyle_hip_op_desc &r, Desc *outs, uint32_t *out_count) {
+  const Desc *in = r.inputs;
+  hyle_hip_status s;
+  if ((s = expect_inputs(r, 4, 4)) != HYLE_HIP_OK) return s;
+  const Desc &query = in[0], &bounds = in[1], &table = in[2], &lengths = in[3];
+  if (!is_floating(query.dtype) || query.rank < 3 || query.rank > 4)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedSelect requires floating queries [sequences, rows, heads, depth] or [sequences, heads, depth]");
+  const int64_t query_heads = query.dims[query.rank - 2], depth = query.dims[query.rank - 1], rows = query.rank == 4 ? query.dims[1] : 1;
+  if (bounds.dtype != HYLE_HIP_DTYPE_BF16 || bounds.rank != 4 || bounds.dims[1] != 2 || bounds.dims[3] != depth)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedSelect requires bfloat16 bounds [pages, 2, heads, depth] of the queries' depth");
+  if (bounds.dims[2] <= 0 || depth <= 0 || query_heads <= 0 || query_heads % bounds.dims[2] != 0)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedSelect requires a positive depth and query heads that are a multiple of the key heads");
+  if (table.dtype != HYLE_HIP_DTYPE_I32 || table.rank != 2 || lengths.dtype != HYLE_HIP_DTYPE_I32 || lengths.rank != 1 ||
+      table.dims[0] != query.dims[0] || lengths.dims[0] != query.dims[0])
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedSelect requires i32 pages [sequences, columns] and i32 lengths [sequences]");
+  const int64_t most = std::numeric_limits<int32_t>::max();
+  if (r.axis <= 0 || rows < 1 || rows > most)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedSelect requires a positive page size and new rows");
+  // the first page, and those that the newest tokens can lie in
+  const int64_t always = 1 + (rows + r.axis - 2) / r.axis + 1;
+  if (r.count > (uint64_t)most || (int64_t)r.count < always)
+    return fail(HYLE_HIP_INVALID_ARGUMENT, "PagedSelect requires a count of at least %lld: the first page and those of the newest tokens", (long long)always);
+  const int64_t dims[3] = {query.dims[0], bounds.dims[2], (int64_t)r.count};
+  *out_count = 2;
+  if ((s = make_dense(HYLE_HIP_DTYPE_I32, dims, 3, &outs[0])) != HYLE_HIP_OK) return s;
+  return make_dense(HYLE_HIP_DTYPE_I32, dims, 2, &outs[1]);
 }
 
 hyle_hip_status infer(const hyle_hip_op_desc &r, Desc *outs, uint32_t *out_count) {
@@ -692,6 +776,9 @@ hyle_hip_status infer(const hyle_hip_op_desc &r, Desc *outs, uint32_t *out_count
     case HYLE_HIP_OP_ATTENTION:
     case HYLE_HIP_OP_PAGED_ATTENTION: return infer_attention(r, outs, out_count);
     case HYLE_HIP_OP_PAGED_APPEND: return infer_paged_append(r, outs);
+    case HYLE_HIP_OP_ROTARY_APPEND: return infer_rotary_append(r, outs, out_count);
+    case HYLE_HIP_OP_PAGE_BOUNDS: return infer_page_bounds(r, outs);
+    case HYLE_HIP_OP_PAGED_SELECT: return infer_paged_select(r, outs, out_count);
     default:
       return fail(HYLE_HIP_UNIMPLEMENTED, "operation kind %u is not served by this provider", r.op);
   }
@@ -723,6 +810,9 @@ enum class Route : uint8_t {
   kRope,
   kAttention,
   kPagedAppend,
+  kRotaryAppend,
+  kPageBounds,
+  kPagedSelect,
 };
 
 const char *route_name(Route r) {
@@ -749,6 +839,9 @@ const char *route_name(Route r) {
     case Route::kRope: return "rope-rows";
     case Route::kAttention: return "attention";
     case Route::kPagedAppend: return "paged-append";
+    case Route::kRotaryAppend: return "rotary-append";
+    case Route::kPageBounds: return "page-bounds";
+    case Route::kPagedSelect: return "paged-select";
   }
   return "?";
 }
@@ -804,7 +897,10 @@ struct hyle_hip_plan {
   AttentionSplit attention_split;
   bool attention_few_rows = false;  // the kernel that splits over the keys, where it serves the operands
   AppendParams append;
-  // Concat, Gather, Attention and PagedAppend take no alias and no overlap: bytes each input spans, for the launch's check
+  RotaryAppendParams rotary_append;
+  PageBoundsParams page_bounds;
+  PagedSelectParams paged_select;
+  // Concat, Gather, Attention, the cache's operations take no alias and no overlap: bytes each input spans, for the launch's check
   uint64_t concat_input_bytes[HYLE_HIP_MAX_INPUTS] = {0, 0, 0, 0};
   // Cast and Copy take no alias at all (AliasPolicy::kNone, src/compute_ops/operation.cc:935-957):
   // the bytes the input and the output occupy must not overlap.
@@ -941,6 +1037,15 @@ bool has_element_rows(const Desc &d) {
   return true;
 }
 
+// A cache of 4 bits keeps a page's rows of one head and side as one run of bytes.
+bool has_whole_pages(const Desc &cache) {
+  if (cache.dtype != HYLE_HIP_DTYPE_U8 || has_zero_extent(cache)) return true;
+  return cache.dims[3] == 1 || cache.byte_strides[3] == cache.dims[4];
+}
+CacheKind cache_kind(uint32_t dtype) {
+  return dtype == HYLE_HIP_DTYPE_U8 ? CacheKind::kFourBits : dtype == HYLE_HIP_DTYPE_F8_E4M3FN ? CacheKind::kNarrow : CacheKind::kKept;
+}
+
 hyle_hip_status admit_attention(hyle_hip_plan *p, uint32_t units) {
   const hyle_hip_op_desc &r = p->request;
   const Desc *in = r.inputs;
@@ -972,23 +1077,40 @@ hyle_hip_status admit_attention(hyle_hip_plan *p, uint32_t units) {
   a.q_row = batched ? query.byte_strides[1] : paged ? 0 : query.byte_strides[0];
   a.q_head = query.byte_strides[query.rank - 2];
   if (paged) {
-    const Desc &cache = in[1], &table = in[2];
+    const Desc &cache = in[1], &table = in[2], &lengths = in[3];
+    const int64_t columns = table.dims[table.rank - 1], heads = cache.dims[2];
     a.sequences = (int32_t)query.dims[0];
     a.rows = batched ? (int32_t)query.dims[1] : 1;
     a.narrow_cache = cache.dtype == HYLE_HIP_DTYPE_F8_E4M3FN;
-    a.heads = (int32_t)cache.dims[2];
-    if (cache.dims[0] > most || table.dims[1] > most || (cache.dims[3] != 0 && table.dims[1] > most / cache.dims[3]))
+    a.four_bits = cache.dtype == HYLE_HIP_DTYPE_U8;
+    a.heads = (int32_t)heads;
+    if (cache.dims[0] > most || columns > most || (cache.dims[3] != 0 && columns > most / cache.dims[3]))
       return fail(HYLE_HIP_UNIMPLEMENTED, "paged attention requires pages and positions within int32");
+    if (!has_whole_pages(cache)) return fail(HYLE_HIP_UNIMPLEMENTED, "a cache of 4 bits requires rows of a page behind one another");
+    if (table.rank == 3) {
+      // each key head of a sequence is a sequence of the kernels
+      if (columns != 0 && ((heads > 1 && query.dims[0] > 1 && table.byte_strides[0] != heads * table.byte_strides[1]) || !is_dense(lengths)))
+        return fail(HYLE_HIP_UNIMPLEMENTED, "paged attention requires pages of key heads at one stride and dense lengths");
+      a.sequences *= a.heads;
+      a.apart = Divisor((uint32_t)heads);
+      a.heads = 1;
+      a.table_row = (heads > 1 ? table.byte_strides[1] : table.byte_strides[0]) / 4;
+    } else {
+      a.table_row = table.byte_strides[0] / 4;
+    }
     a.pages = (int32_t)cache.dims[0];
-    a.columns = (int32_t)table.dims[1];
-    a.table_row = table.byte_strides[0] / 4;
-    a.keys = a.pages == 0 ? 0 : (int32_t)(table.dims[1] * cache.dims[3]);
+    a.columns = (int32_t)columns;
+    a.keys = a.pages == 0 ? 0 : (int32_t)(columns * cache.dims[3]);
     a.page = Divisor(cache.dims[3] > 0 ? (uint32_t)cache.dims[3] : 1u);
     a.k_sequence = cache.byte_strides[0];
     a.k_head = cache.byte_strides[2];
     a.k_row = cache.byte_strides[3];
     a.v_sequence = a.k_sequence, a.v_head = a.k_head, a.v_row = a.k_row;
     a.value_offset = cache.byte_strides[1];
+    if (a.four_bits) {
+      a.k_row = a.v_row = depth / 2;
+      a.scale_offset = cache.dims[3] * (depth / 2);
+    }
   } else {
     const Desc &key = in[1], &value = in[2];
     const int row = batched ? 1 : 0;
@@ -1008,7 +1130,7 @@ hyle_hip_status admit_attention(hyle_hip_plan *p, uint32_t units) {
     if ((uint64_t)a.sequences * (uint64_t)a.queries > kMaxElements / 2)
       return fail(HYLE_HIP_UNIMPLEMENTED, "attention requires at most INT32_MAX / 2 heads of sequences");
   }
-  a.shared = Divisor((uint32_t)(a.queries / a.heads));
+  a.shared = Divisor((uint32_t)(a.queries / (a.heads * (int32_t)a.apart.divisor)));
   for (uint32_t i = 0; i < r.input_count; ++i) p->concat_input_bytes[i] = spanned_bytes(in[i]);
   p->route = Route::kAttention;
   p->dispatches = 1;
@@ -1047,12 +1169,118 @@ hyle_hip_status admit_paged_append(hyle_hip_plan *p) {
   a.depth = (uint32_t)in[0].dims[2];
   a.pages = (uint32_t)p->request.count;
   a.page = Divisor((uint32_t)p->request.axis);
-  a.narrow_cache = p->request.kind == HYLE_HIP_DTYPE_F8_E4M3FN;
+  a.cache = cache_kind(p->request.kind);
   a.k_token = in[0].byte_strides[0], a.k_head = in[0].byte_strides[1];
   a.v_token = in[1].byte_strides[0], a.v_head = in[1].byte_strides[1];
   for (int i = 0; i < 3; ++i) p->concat_input_bytes[i] = spanned_bytes(in[i]);
   p->route = Route::kPagedAppend;
   p->dispatches = 1;
+  return HYLE_HIP_OK;
+}
+
+hyle_hip_status admit_rotary_append(hyle_hip_plan *p) {
+  const hyle_hip_op_desc &r = p->request;
+  const Desc *in = r.inputs;
+  if (!to_elem(in[0].dtype, &p->elem)) return fail(HYLE_HIP_UNIMPLEMENTED, "RotaryAppend requires float32/float16/bfloat16 rows");
+  for (int i = 0; i < 4; ++i)
+    if (i == 0 ? !has_element_rows(in[i]) : !is_plain(in[i]) || !is_dense(in[i]))
+      return fail(HYLE_HIP_UNIMPLEMENTED, "RotaryAppend requires rows with a dense last axis and whole elements to a stride, and dense positions, frequencies and slots");
+  if (in[0].dims[2] > 1024) return fail(HYLE_HIP_UNIMPLEMENTED, "RotaryAppend serves depths up to 1024");
+  if (p->input_elements[0] > kMaxElements) return fail(HYLE_HIP_UNIMPLEMENTED, "RotaryAppend requires at most INT32_MAX elements");
+  if (!axis_holds((uint64_t)in[0].dims[0] * (uint64_t)in[0].dims[1] / 4 + 1, 256))
+    return fail(HYLE_HIP_UNIMPLEMENTED, "RotaryAppend requires at most 2^26 heads of tokens to a launch");
+  if (p->input_elements[0] == 0 || (p->output_elements[0] == 0 && p->output_count == 1)) return HYLE_HIP_OK;
+  RotaryAppendParams &a = p->rotary_append;
+  a.tokens = (uint32_t)in[0].dims[0];
+  a.heads = (uint32_t)r.axes[0];
+  a.queries = (uint32_t)in[0].dims[1] - 2 * a.heads;
+  a.depth = (uint32_t)in[0].dims[2];
+  a.rotary = 2 * (uint32_t)in[2].dims[in[2].rank - 1];
+  a.pages = (uint32_t)r.count;
+  a.page = Divisor((uint32_t)r.axis);
+  a.half_split = r.kind2 == HYLE_HIP_ROPE_HALF_SPLIT;
+  a.wide_positions = in[1].dtype == HYLE_HIP_DTYPE_I64;
+  a.stepped_frequencies = in[2].rank == 2;
+  a.cache = cache_kind(r.kind);
+  a.token = in[0].byte_strides[0], a.head = in[0].byte_strides[1];
+  for (int i = 0; i < 4; ++i) p->concat_input_bytes[i] = spanned_bytes(in[i]);
+  p->route = Route::kRotaryAppend;
+  p->dispatches = 1;
+  return HYLE_HIP_OK;
+}
+
+hyle_hip_status admit_page_bounds(hyle_hip_plan *p) {
+  const hyle_hip_op_desc &r = p->request;
+  const Desc &cache = r.inputs[0], &table = r.inputs[1];
+  PageBoundsParams &a = p->page_bounds;
+  a.cache = cache_kind(cache.dtype);
+  if (a.cache == CacheKind::kKept && !to_elem(cache.dtype, &a.type))
+    return fail(HYLE_HIP_UNIMPLEMENTED, "PageBounds requires a cache of float32/float16/bfloat16, float8 e4m3 or 4 bits");
+  for (int i = 0; i < 3; ++i)
+    if (!has_element_rows(r.inputs[i]))
+      return fail(HYLE_HIP_UNIMPLEMENTED, "PageBounds requires plain operands with a dense last axis and whole elements to a stride");
+  if (!has_whole_pages(cache)) return fail(HYLE_HIP_UNIMPLEMENTED, "a cache of 4 bits requires rows of a page behind one another");
+  if (p->output_elements[0] == 0 || p->input_elements[0] == 0 || p->input_elements[1] == 0) return HYLE_HIP_OK;
+  const uint64_t heads = (uint64_t)cache.dims[2], depth = (uint64_t)cached_depth(cache), page = (uint64_t)cache.dims[3];
+  if ((uint64_t)cache.dims[0] > kMaxElements || page > kMaxElements || depth * heads > kMaxElements || (uint64_t)table.dims[1] > kMaxElements)
+    return fail(HYLE_HIP_UNIMPLEMENTED, "PageBounds requires pages, rows and channels within int32");
+  a.sequences = (uint32_t)table.dims[0], a.columns = (uint32_t)table.dims[1];
+  a.heads = (uint32_t)heads, a.depth = (uint32_t)depth, a.pages = (uint32_t)cache.dims[0];
+  a.newest = (uint32_t)r.count;
+  const uint64_t span = a.newest == 0 ? a.columns : (a.newest + page - 2) / page + 1;
+  a.span = (uint32_t)(span < a.columns ? span : a.columns);
+  if ((uint64_t)table.dims[0] > kMaxElements || !axis_holds((uint64_t)a.sequences * a.span, 256) || !axis_holds((uint64_t)a.sequences * a.span * heads, 256))
+    return fail(HYLE_HIP_UNIMPLEMENTED, "PageBounds requires at most 2^24 pages of key heads to a launch");
+  a.page_bytes = cache.byte_strides[0], a.head_bytes = cache.byte_strides[2];
+  a.row_bytes = a.cache == CacheKind::kFourBits ? (int64_t)depth / 2 : cache.byte_strides[3];
+  a.scale_offset = (int64_t)(page * (depth / 2));
+  a.table_row = table.byte_strides[0] / 4;
+  a.page = Divisor((uint32_t)page);
+  for (int i = 0; i < 3; ++i) p->concat_input_bytes[i] = spanned_bytes(r.inputs[i]);
+  p->route = Route::kPageBounds;
+  p->dispatches = 1;
+  return HYLE_HIP_OK;
+}
+
+hyle_hip_status admit_paged_select(hyle_hip_plan *p) {
+  const hyle_hip_op_desc &r = p->request;
+  const Desc &query = r.inputs[0], &bounds = r.inputs[1], &table = r.inputs[2];
+  if (!to_elem(query.dtype, &p->elem)) return fail(HYLE_HIP_UNIMPLEMENTED, "PagedSelect requires float32/float16/bfloat16 queries");
+  for (int i = 0; i < 4; ++i)
+    if (!has_element_rows(r.inputs[i]))
+      return fail(HYLE_HIP_UNIMPLEMENTED, "PagedSelect requires plain operands with a dense last axis and whole elements to a stride");
+  const int64_t depth = query.dims[query.rank - 1], most = std::numeric_limits<int32_t>::max();
+  if (depth > 256) return fail(HYLE_HIP_UNIMPLEMENTED, "PagedSelect serves depths up to 256");
+  if (p->output_elements[0] > kMaxElements || p->input_elements[0] > kMaxElements)
+    return fail(HYLE_HIP_UNIMPLEMENTED, "PagedSelect requires at most INT32_MAX chosen pages and query elements");
+  if (bounds.dims[0] > most || table.dims[1] > most / r.axis)
+    return fail(HYLE_HIP_UNIMPLEMENTED, "PagedSelect requires pages and positions within int32");
+  if (p->output_elements[0] == 0) return HYLE_HIP_OK;
+  PagedSelectParams &a = p->paged_select;
+  const bool batched = query.rank == 4;
+  a.sequences = (uint32_t)query.dims[0];
+  a.rows = batched ? (uint32_t)query.dims[1] : 1u;
+  a.queries = (uint32_t)query.dims[query.rank - 2];
+  a.heads = (uint32_t)bounds.dims[2];
+  a.depth = (uint32_t)depth;
+  a.pages = (uint32_t)bounds.dims[0];
+  a.columns = (uint32_t)table.dims[1];
+  a.count = (uint32_t)r.count;
+  a.q_sequence = query.byte_strides[0];
+  a.q_row = batched ? query.byte_strides[1] : 0;
+  a.q_head = query.byte_strides[query.rank - 2];
+  a.b_page = bounds.byte_strides[0], a.b_side = bounds.byte_strides[1], a.b_head = bounds.byte_strides[2];
+  a.table_row = table.byte_strides[0] / 4;
+  a.page = Divisor((uint32_t)r.axis);
+  a.shared = Divisor(a.queries / a.heads);
+  const uint64_t lines = (uint64_t)a.sequences * a.heads, scored = a.columns > a.count ? lines * a.columns : 0;
+  if (!axis_holds(lines, 1024) || !axis_holds((scored + 3) / 4, 256))
+    return fail(HYLE_HIP_UNIMPLEMENTED, "PagedSelect requires at most 2^22 key heads of sequences and 2^26 pages of them to a launch");
+  for (int i = 0; i < 4; ++i) p->concat_input_bytes[i] = spanned_bytes(r.inputs[i]);
+  p->workspace_size = scored * sizeof(uint32_t);
+  p->workspace_alignment = scored != 0 ? 256 : 1;
+  p->route = Route::kPagedSelect;
+  p->dispatches = scored != 0 ? 2 : 1;
   return HYLE_HIP_OK;
 }
 
@@ -1611,6 +1839,9 @@ hyle_hip_status admit(hyle_hip_plan *p) {
     case HYLE_HIP_OP_ATTENTION:
     case HYLE_HIP_OP_PAGED_ATTENTION: return admit_attention(p, units);
     case HYLE_HIP_OP_PAGED_APPEND: return admit_paged_append(p);
+    case HYLE_HIP_OP_ROTARY_APPEND: return admit_rotary_append(p);
+    case HYLE_HIP_OP_PAGE_BOUNDS: return admit_page_bounds(p);
+    case HYLE_HIP_OP_PAGED_SELECT: return admit_paged_select(p);
     case HYLE_HIP_OP_COPY:
     case HYLE_HIP_OP_CAST: {
       // src/compute_provider_native/cast.cc:127-176,256-279 (admitted pairs, plain input, dense
@@ -2104,7 +2335,8 @@ hyle_hip_status hyle_hip_plan_launch(const hyle_hip_plan *plan, const void *cons
       b.marks = input_count > 3 ? static_cast<const int32_t *>(inputs[3]) : nullptr;
       b.out = outputs[0];
       b.logs = output_count > 1 ? static_cast<float *>(outputs[1]) : nullptr;
-      const bool vectors = aligned(inputs[0], 16) && aligned(inputs[1], 16) && aligned(b.value, 16) && aligned(b.out, 16);
+      const size_t keys = plan->attention.four_bits ? 4 : 16;
+      const bool vectors = aligned(inputs[0], 16) && aligned(inputs[1], keys) && aligned(b.value, keys) && aligned(b.out, 16);
       if (plan->attention_few_rows && attention_split_serves(plan->elem, plan->attention, vectors))
         err = launch_attention_split(plan->elem, plan->attention, b, plan->attention_split, workspace, stream);
       else if (attention_tiles_serves(plan->elem, plan->attention, vectors)) err = launch_attention_tiles(plan->elem, plan->attention, b, plan->context->compute_units, stream);
@@ -2115,6 +2347,23 @@ hyle_hip_status hyle_hip_plan_launch(const hyle_hip_plan *plan, const void *cons
       if ((s = refuse_overlaps(plan, inputs, outputs, "PagedAppend")) != HYLE_HIP_OK) return s;
       err = launch_paged_append(plan->elem, plan->append, inputs[0], inputs[1], static_cast<const int32_t *>(inputs[2]), outputs[0],
                                 aligned(inputs[0], 16) && aligned(inputs[1], 16) && aligned(outputs[0], 16), stream);
+      break;
+    case Route::kRotaryAppend:
+      if ((s = refuse_overlaps(plan, inputs, outputs, "RotaryAppend")) != HYLE_HIP_OK) return s;
+      err = launch_rotary_append(plan->elem, plan->rotary_append, inputs[0], inputs[1], inputs[2], static_cast<const int32_t *>(inputs[3]),
+                                 outputs[0], output_count > 1 ? outputs[1] : nullptr,
+                                 aligned(inputs[0], 16) && aligned(outputs[0], 16) && (output_count < 2 || aligned(outputs[1], 16)), stream);
+      break;
+    case Route::kPageBounds:
+      if ((s = refuse_overlaps(plan, inputs, outputs, "PageBounds")) != HYLE_HIP_OK) return s;
+      err = launch_page_bounds(plan->page_bounds, inputs[0], static_cast<const int32_t *>(inputs[1]), static_cast<const int32_t *>(inputs[2]),
+                               outputs[0], aligned(inputs[0], 16) && aligned(outputs[0], 16), stream);
+      break;
+    case Route::kPagedSelect:
+      if ((s = refuse_overlaps(plan, inputs, outputs, "PagedSelect")) != HYLE_HIP_OK) return s;
+      err = launch_paged_select(plan->elem, plan->paged_select, inputs[0], inputs[1], static_cast<const int32_t *>(inputs[2]),
+                                static_cast<const int32_t *>(inputs[3]), static_cast<int32_t *>(outputs[0]), static_cast<int32_t *>(outputs[1]),
+                                workspace, aligned(inputs[0], 16) && aligned(inputs[1], 16), stream);
       break;
     case Route::kRandomBits:
       err = launch_random_bits(plan->random_bits, inputs[0], outputs[0], stream);

@@ -186,18 +186,56 @@ typedef enum hyle_hip_op_kind {
   HYLE_HIP_OP_ATTENTION = 0x105,
   /* The same for the newest tokens of each sequence against a paged cache: in0 queries [B, R, Hq, D] or [B, Hq, D]
    * (R = 1), in1 the cache [P, 2, H, page, D] (keys at 0, values at 1 of the second axis; in0's type or F8_E4M3FN,
-   * whose elements are the values themselves), in2 I32 [B, M] pages of each sequence in order, in3 I32 [B] lengths:
+   * whose elements are the values themselves, or 4 bits, see below), in2 I32 [B, M] pages of each sequence in order, in3 I32 [B] lengths:
    * the keys of each sequence, the new tokens' own among them (keys past M * page do not exist).  Query i stands at
    * position in3 - R + i.  A page outside [0, P) holds no keys and is never read.  `scale`, `count`, `axis` and
    * `kind2` as for ATTENTION; always causal.  A contiguous cache is one page per sequence.  Made for a few new
-   * tokens: of R in the hundreds, every 64 rows of a key head read all keys that any row of their sequence sees. */
+   * tokens: of R in the hundreds, every 64 rows of a key head read all keys that any row of their sequence sees.
+   *   Pages chosen for each key head (PAGED_SELECT): in2 I32 [B, H, M] and in3 I32 [B, H], dense; each key head of a
+   *     sequence has pages and a length of its own, and places and windows are counted in those.
+   *   4 bits: the cache is U8 [P, 2, H, page, 17 D / 32], D a multiple of 32.  The bytes of a head's side of a page
+   *     stand behind one another: the codes [page, D / 2] of its rows, the first of two elements in the low bits,
+   *     then their scales [page, D / 32], one to 32 neighbours along the depth.  A code is a sign, two exponent bits
+   *     and one of mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6) and stands for that number times 2^(scale - 127); a scale of
+   *     255 makes its elements NaN.  (Under f16 queries values beyond 65504 are infinite.) */
   HYLE_HIP_OP_PAGED_ATTENTION = 0x106,
   /* Keys and values of new tokens into such a cache: in0 keys, in1 values [T, H, D] of one type, in2 I32 [T] slots
    * (page * page size + place in the page).  out0 is the cache, dense [P, 2, H, page, D]: `count` = P, `axis` = page
    * size, `kind` = its type (in0's or F8_E4M3FN: nearest even, beyond +-448 the nearest end, NaN stays).  Only the
    * tokens' rows are written.  A slot outside the cache writes nothing.  Slots inside it should differ: one that
-   * several tokens have ends with elements of any of them, each as one of them has it at that place. */
-  HYLE_HIP_OP_PAGED_APPEND = 0x107
+   * several tokens have ends with elements of any of them, each as one of them has it at that place.
+   *   `kind` = U8 keeps 4 bits (PAGED_ATTENTION has the layout; D a multiple of 32): the scale of 32 elements is the
+   *   power of two two below their largest magnitude's, doubled where its significand is over 1.75, within 2^-127 and
+   *   2^125 (2^13 of F16 tokens); codes are nearest, ties to even, beyond 6 scales the nearest end; an infinity or NaN
+   *   makes its 32 elements NaN.  (A slot of several tokens ends with codes and scales of any of them.) */
+  HYLE_HIP_OP_PAGED_APPEND = 0x107,
+  /* The projection of new tokens rotated by their positions on the way to the cache: ROPE of queries and keys, and
+   * PAGED_APPEND.  in0 [T, Hq + 2 H, D] (F32 / F16 / BF16, any byte strides but a dense last axis; D up to 1024): Hq
+   * query heads, then H key heads, then H value heads; in1 dense I32 / I64 [T] positions; in2 dense F32 frequencies
+   * [rotary / 2] or [T, rotary / 2]; in3 dense I32 [T] slots.  `axes_count` = 1 and axes[0] = H; `kind2` =
+   * hyle_hip_rope_layout; `count`, `axis`, `kind` and out0 as for PAGED_APPEND; with Hq > 0 out1 holds the rotated
+   * queries, dense [T, Hq, D] of in0's type, those of tokens without a slot among them.  cos and sin are those of the f32 phase
+   * rounded to f32 from 64 bits; the rotation is in f32, each product and sum rounded, and an element is rounded once more, to what
+   * keeps it.  Elements past the rotary width and values are only stored. */
+  HYLE_HIP_OP_ROTARY_APPEND = 0x108,
+  /* What the keys of a page lie within: in0 a cache as for PAGED_ATTENTION (of any of its types), in1 I32 [B, M] pages,
+   * in2 I32 [B] lengths; out0 BF16 [P, 2, H, D]: of each page, key head and channel the least key at 0 and the largest at 1
+   * of the second axis, a number that bf16 lacks as the next one below or above.  Elements that are no numbers have no part
+   * (a channel of none holds +inf and -inf).  `count` = newest tokens: the pages of each sequence that hold one of its
+   * last `count` tokens are written, from all keys that it has in them; 0 writes all of its pages.  Others stay as
+   * they were, and a page outside [0, P) is none.  A page of two sequences should hold as many keys of both: its bounds
+   * are those of one of them, channel by channel. */
+  HYLE_HIP_OP_PAGE_BOUNDS = 0x109,
+  /* The pages of each key head whose keys may have the largest products with its queries: in0 queries as for
+   * PAGED_ATTENTION, in1 BF16 [P, 2, H, D] bounds (PAGE_BOUNDS), in2 I32 [B, M] pages, in3 I32 [B] lengths; `axis` = page size,
+   * `count` = K, the pages to choose.  A page's score for a key head is the largest, over its query heads and the new
+   * rows, of the sum over d of q_d * (q_d >= 0 ? largest_d : least_d), summed in f64 and rounded to f32; one that is no number
+   * counts as +inf, that of a page outside [0, P) as -inf.  The sequence's first page and those of its R newest tokens are
+   * always chosen (K is at least 1 + (R + axis - 2) / axis + 1), then those of the highest scores, of equal ones the
+   * earlier.  out0 I32 [B, H, K]: the chosen pages in their order, -1 behind them; out1 I32 [B, H]: the keys in them,
+   * the sequence's length less `axis` for every page that was not chosen.  Both are what PAGED_ATTENTION takes for each
+   * key head; the new tokens are the last of them.  Two dispatches and a workspace, one where M <= K. */
+  HYLE_HIP_OP_PAGED_SELECT = 0x10A
 } hyle_hip_op_kind;
 
 /* UnaryKind (include/hyle/compute/operation.h:57-73) */
@@ -266,14 +304,14 @@ typedef struct hyle_hip_tensor_desc {
 typedef struct hyle_hip_op_desc {
   uint32_t abi_version;      /* HYLE_HIP_ABI_VERSION */
   uint32_t op;               /* hyle_hip_op_kind */
-  uint32_t kind;             /* Unary/Binary/Reduction/GatedActivation kind; Cast, Fill, PagedAppend: output hyle_hip_dtype;
+  uint32_t kind;             /* Unary/Binary/Reduction/GatedActivation kind; Cast, Fill, PagedAppend, RotaryAppend: output hyle_hip_dtype;
                                 Attention: 1 = causal */
   uint32_t kind2;            /* BINARY_CHAIN: second BinaryKind; GATED: GatedInputKind;
                                 SOFTMAX: SoftmaxKind; GGUF_MATVEC: HYLE_HIP_ACTIVATIONS_*;
                                 GATHER: hyle_hip_index_bounds; CATEGORICAL: 1 = also log probabilities;
-                                ROPE: hyle_hip_rope_layout; ATTENTION, PAGED_ATTENTION: 1 = also the rows' logarithms */
+                                ROPE, ROTARY_APPEND: hyle_hip_rope_layout; ATTENTION, PAGED_ATTENTION: 1 = also the rows' logarithms */
   int32_t axis;              /* Softmax / TopK / Concat / Gather axis, RoPE sequence axis (negative counts from the end);
-                                Attention, PagedAttention: sinks; PagedAppend: page size */
+                                Attention, PagedAttention: sinks; PagedAppend, RotaryAppend, PagedSelect: page size */
   uint32_t mask;             /* Softmax MaskKind */
   uint32_t accumulation;     /* hyle_hip_dtype; UNKNOWN or F32 */
   uint32_t keep_dimensions;  /* Reduce */
@@ -281,14 +319,14 @@ typedef struct hyle_hip_op_desc {
   float scale;               /* Softmax, Attention, PagedAttention */
   uint64_t count;            /* TopK count; Fill: the scalar's bits; Concat: the group's start on the axis;
                                 RandomBits: word_count; RoPE: rotary_dimensions; Attention, PagedAttention:
-                                window; PagedAppend: pages */
+                                window; PagedAppend, RotaryAppend: pages; PageBounds: newest tokens; PagedSelect: pages to choose */
   uint32_t largest;          /* TopK: 1 = largest first, 0 = smallest first */
   uint32_t input_count;
   hyle_hip_tensor_desc inputs[HYLE_HIP_MAX_INPUTS];
   /* Reduce::axes (include/hyle/compute/operation.h:232-247, 307-312): axes_count = 0 is
    * Axes::all(); otherwise the first axes_count entries of `axes`, each possibly negative
    * (counted from the end); a duplicate is INVALID_ARGUMENT as in the schema
-   * (src/compute_ops/operation.cc:1358-1377). */
+   * (src/compute_ops/operation.cc:1358-1377).  RotaryAppend: one entry, the key heads. */
   uint32_t axes_count;
   int32_t axes[HYLE_HIP_MAX_RANK];
 } hyle_hip_op_desc;

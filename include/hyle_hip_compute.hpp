@@ -366,9 +366,21 @@ struct Attention final {
 };
 struct PagedAttention final { float scale = 1.0F; std::uint32_t window = 0; std::int32_t sinks = 0; bool return_log_sum = false; };
 struct PagedAppend final { std::size_t pages = 0; std::int32_t page_size = 0; DataType cache_type = DataType::kUnknown; };
+// PagedAppend of projected rows whose queries and keys are rotated on the way, and the choice of the pages that PagedAttention
+// reads for each key head (HYLE_HIP_OP_ROTARY_APPEND, _PAGE_BOUNDS and _PAGED_SELECT).
+struct RotaryAppend final {
+  std::size_t pages = 0;
+  std::int32_t page_size = 0;
+  DataType cache_type = DataType::kUnknown;
+  std::int32_t key_heads = 0;
+  RopeLayout layout = RopeLayout::kInterleaved;
+};
+struct PageBounds final { std::uint32_t newest = 0; };
+struct PagedSelect final { std::uint32_t count = 0; std::int32_t page_size = 0; };
 
 using Operation = std::variant<Copy, Fill, Select, Concat, Gather, Cast, Unary, Binary, Reduce, RmsNorm, LayerNorm, GatedActivation, Softmax, TopK, BinaryChain,
-                               Q8_0DequantSumSquares, GgufMatVec, RandomBits, Categorical, RoPE, Attention, PagedAttention, PagedAppend>;
+                               Q8_0DequantSumSquares, GgufMatVec, RandomBits, Categorical, RoPE, Attention, PagedAttention, PagedAppend,
+                               RotaryAppend, PageBounds, PagedSelect>;
 
 namespace detail {
 inline hyle_hip_op_desc to_c(const Operation &operation, const TensorDesc *inputs, std::size_t count) noexcept {
@@ -439,6 +451,12 @@ inline hyle_hip_op_desc to_c(const Operation &operation, const TensorDesc *input
     void operator()(const PagedAppend &o) const {
       r.op = HYLE_HIP_OP_PAGED_APPEND; r.kind = static_cast<std::uint32_t>(o.cache_type); r.count = o.pages; r.axis = o.page_size;
     }
+    void operator()(const RotaryAppend &o) const {
+      r.op = HYLE_HIP_OP_ROTARY_APPEND; r.kind = static_cast<std::uint32_t>(o.cache_type); r.count = o.pages; r.axis = o.page_size;
+      r.kind2 = static_cast<std::uint32_t>(o.layout); r.axes_count = 1; r.axes[0] = o.key_heads;
+    }
+    void operator()(const PageBounds &o) const { r.op = HYLE_HIP_OP_PAGE_BOUNDS; r.count = o.newest; }
+    void operator()(const PagedSelect &o) const { r.op = HYLE_HIP_OP_PAGED_SELECT; r.count = o.count; r.axis = o.page_size; }
     void operator()(const Categorical &o) const { r.op = HYLE_HIP_OP_CATEGORICAL; r.kind2 = o.return_log_probability ? 1u : 0u; }
   };
   std::visit(Fill{r}, operation);

@@ -25,7 +25,7 @@ def pytest_configure(config):
 
 
 # Modules whose cases reach launch shapes that no other module does, beside those that the coverage test itself asks for.
-COVERAGE_MODULES = ("test_gpu_attention", "test_gpu_paged_attention")
+COVERAGE_MODULES = ("test_gpu_attention", "test_gpu_paged_attention", "test_gpu_cache_operators")
 
 
 def pytest_collection_modifyitems(items):

@@ -238,6 +238,28 @@ HOST_TEST(AttentionAndItsCacheFollowTheSchema) {
   EXPECT((*out)[0] == cache);
 }
 
+HOST_TEST(TheCacheOfADecodingStepFollowsTheSchema) {
+  const TensorDesc places = dense(DataType::kInt32, {7}), rows = dense(DataType::kFloat16, {7, 12, 64});
+  auto out = infer_output_descriptions(RotaryAppend{.pages = 10, .page_size = 16, .cache_type = DataType::kUInt8, .key_heads = 2, .layout = RopeLayout::kHalfSplit},
+                                       {rows, places, dense(DataType::kFloat32, {32}), places});
+  const TensorDesc cache = dense(DataType::kUInt8, {10, 2, 2, 16, 34}), query = dense(DataType::kFloat16, {7, 8, 64});
+  REQUIRE(out.has_value() && out->size() == 2);
+  EXPECT((*out)[0] == cache && (*out)[1] == query);
+  const TensorDesc pages = dense(DataType::kInt32, {7, 5}), bounds = dense(DataType::kBFloat16, {10, 2, 2, 64});
+  out = infer_output_descriptions(PageBounds{.newest = 1}, {cache, pages, places});
+  REQUIRE(out.has_value() && out->size() == 1);
+  EXPECT((*out)[0] == bounds);
+  out = infer_output_descriptions(PagedSelect{.count = 4, .page_size = 16}, {query, bounds, pages, places});
+  REQUIRE(out.has_value() && out->size() == 2);
+  EXPECT((*out)[0] == dense(DataType::kInt32, {7, 2, 4}) && (*out)[1] == dense(DataType::kInt32, {7, 2}));
+  out = infer_output_descriptions(PagedAttention{}, {query, cache, (*out)[0], (*out)[1]});
+  REQUIRE(out.has_value() && out->size() == 1);
+  EXPECT((*out)[0] == query);
+  EXPECT(infer_output_descriptions(PagedSelect{.count = 1, .page_size = 16}, {query, bounds, pages, places}).error().IsInvalidArgument());
+  EXPECT(infer_output_descriptions(RotaryAppend{.pages = 10, .page_size = 16, .cache_type = DataType::kUInt8, .key_heads = 7},
+                                   {rows, places, dense(DataType::kFloat32, {32}), places}).error().IsInvalidArgument());
+}
+
 HOST_TEST(SubmitWithoutDeviceIsFailedPrecondition) {
   Context context = Context::planning_only();
   EXPECT(context.create_queue().error().IsFailedPrecondition());
@@ -758,6 +780,29 @@ DEVICE_TEST(PagedAttentionReadsWhatPagedAppendWrote) {
   const std::vector<float> kept = download<float>(held, 48);
   for (int i = 0; i < 32; ++i) EXPECT(kept[i] == 7.0F);
   EXPECT(kept[32] == 1.0F && kept[37] == 1.0F && kept[40] == 1.0F && kept[44] == 3.0F);
+}
+
+DEVICE_TEST(RotaryAppendTurnsQueriesAndKeys) {
+  // one query, key and value head of four dims at position 0 (nothing turns) and at a position whose first pair turns by one; the second
+  // token's slot is outside the cache
+  const TensorDesc rows = dense(DataType::kFloat32, {2, 3, 4}), cache = dense(DataType::kFloat32, {1, 2, 1, 2, 4});
+  const TensorDesc places = dense(DataType::kInt32, {2}), rates = dense(DataType::kFloat32, {2}), query = dense(DataType::kFloat32, {2, 1, 4});
+  auto prepared = prepare(fixture().context, RotaryAppend{.pages = 1, .page_size = 2, .cache_type = DataType::kFloat32, .key_heads = 1}, rows, places, rates, places);
+  REQUIRE(prepared.has_value());
+  DeviceBuffer x = upload(std::vector<float>{1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12});
+  DeviceBuffer positions = upload(std::vector<std::int32_t>{0, 4}), turns = upload(std::vector<float>{0.25F, 0.0F}), slots = upload(std::vector<std::int32_t>{1, -1});
+  DeviceBuffer held = upload(std::vector<float>(16, 7.0F)), turned = upload(std::vector<float>(8, 7.0F));
+  auto invocation = prepared->create_invocation();
+  REQUIRE(invocation.has_value());
+  auto done = invocation->submit(fixture().queue, {*ConstTensorView::create(rows, x), *ConstTensorView::create(places, positions),
+                                                   *ConstTensorView::create(rates, turns), *ConstTensorView::create(places, slots)},
+                                 {*TensorView::create(cache, held), *TensorView::create(query, turned)});
+  REQUIRE(done.has_value());
+  EXPECT(done->wait().ok());
+  EXPECT(download<float>(held, 16) == std::vector<float>({7, 7, 7, 7, 5, 6, 7, 8, 7, 7, 7, 7, 9, 10, 11, 12}));
+  const float c = static_cast<float>(std::cos(1.0)), s = static_cast<float>(std::sin(1.0));
+  const std::vector<float> got = download<float>(turned, 8);
+  EXPECT(got == std::vector<float>({1, 2, 3, 4, 1 * c - 2 * s, 1 * s + 2 * c, 3, 4}));
 }
 
 DEVICE_TEST(RejectedSubmissionsEnqueueNothing) {
