@@ -470,6 +470,6 @@ struct PagedSelectParams {
 };
 hipError_t launch_paged_select(Elem type, const PagedSelectParams &p, const void *query, const void *bounds, const int32_t *table,
                                const int32_t *lengths, int32_t *selected, int32_t *seen, void *workspace, bool vector_aligned,
-                               hipStream_t stream);
+                               int compute_units, hipStream_t stream);
 
 }  // namespace hyle_hip

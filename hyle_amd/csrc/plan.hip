@@ -2363,7 +2363,7 @@ hyle_hip_status hyle_hip_plan_launch(const hyle_hip_plan *plan, const void *cons
       if ((s = refuse_overlaps(plan, inputs, outputs, "PagedSelect")) != HYLE_HIP_OK) return s;
       err = launch_paged_select(plan->elem, plan->paged_select, inputs[0], inputs[1], static_cast<const int32_t *>(inputs[2]),
                                 static_cast<const int32_t *>(inputs[3]), static_cast<int32_t *>(outputs[0]), static_cast<int32_t *>(outputs[1]),
-                                workspace, aligned(inputs[0], 16) && aligned(inputs[1], 16), stream);
+                                workspace, aligned(inputs[0], 16) && aligned(inputs[1], 16), (int)plan->context->compute_units, stream);
       break;
     case Route::kRandomBits:
       err = launch_random_bits(plan->random_bits, inputs[0], outputs[0], stream);

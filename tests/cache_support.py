@@ -110,15 +110,13 @@ def selected(query: np.ndarray, bounds: np.ndarray, table: np.ndarray, lengths, 
         newest = min(max(length - rows, 0) // page, filled)
         for h in range(heads):
             score = np.full(filled, -np.inf)
-            for column in range(1, newest):
-                at = table[i, column]
-                if not 0 <= at < bounds.shape[0]:
-                    continue
-                low, high = bounds[at, :, h]
-                with np.errstate(all="ignore"):
-                    sums = [np.float32((q * np.where(q >= 0, high, low)).sum())
-                            for q in query[i, max(rows - length, 0):, h * shared:(h + 1) * shared].reshape(-1, query.shape[-1])]
-                score[column] = max((np.inf if np.isnan(v) else v for v in sums), default=-np.inf)
+            at = table[i, :filled]
+            there = np.flatnonzero((at >= 0) & (at < bounds.shape[0]))
+            low, high = bounds[at[there], 0, h], bounds[at[there], 1, h]
+            with np.errstate(all="ignore"):
+                for q in query[i, max(rows - length, 0):, h * shared:(h + 1) * shared].reshape(-1, query.shape[-1]):
+                    sums = (q * np.where(q >= 0, high, low)).sum(-1).astype(np.float32)
+                    score[there] = np.maximum(score[there], np.where(np.isnan(sums), np.inf, sums))
             always = [c for c in range(filled) if c == 0 or c >= newest]
             others = [c for c in range(filled) if not (c == 0 or c >= newest)]
             others.sort(key=lambda c: (-score[c], c))

@@ -404,6 +404,11 @@ SELECTS = [
     ("bf16", 8, 2, 128, 16, 9, 1, (300, 2000), 2),
     ("f16", 24, 3, 128, 16, 17, 5, (300, 2000, 4), 0),
     ("bf16", 64, 1, 128, 64, 4, 8, (5000, 640), 0),
+    # two and four waves to the query rows, rows that no group of four fills, few and many pages of every depth's kernel, blocks that end inside
+    # a sequence, pages that threads keep in registers and those that they do not
+    ("f16", 7, 1, 64, 16, 9, 1, (3000, 170), 0), ("bf16", 14, 2, 256, 16, 9, 1, (3000, 170), 0), ("f32", 12, 2, 128, 16, 9, 2, (3000, 170), 0),
+    ("bf16", 6, 3, 64, 1, 700, 2, (30011, 29000), 0), ("f16", 5, 1, 128, 1, 30, 3, (40001,), 0), ("bf16", 4, 2, 256, 1, 3000, 1, (9000, 4099, 300), 0),
+    ("f32", 2, 2, 136, 1, 5, 1, (16384, 16385), 0), ("f16", 4, 1, 96, 1, 16000, 1, (17000, 40000), 0),
 ]
 
 
