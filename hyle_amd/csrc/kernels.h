@@ -459,7 +459,7 @@ struct PageBoundsParams {
   Divisor page;
 };
 hipError_t launch_page_bounds(const PageBoundsParams &p, const void *cache, const int32_t *table, const int32_t *lengths, void *bounds,
-                              bool vector_aligned, hipStream_t stream);
+                              hipStream_t stream);
 
 // PagedSelect: scores of pages [sequences, heads, columns] (f32, the workspace), then the best `count` of each key head in order.
 struct PagedSelectParams {

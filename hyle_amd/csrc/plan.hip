@@ -2357,7 +2357,7 @@ hyle_hip_status hyle_hip_plan_launch(const hyle_hip_plan *plan, const void *cons
     case Route::kPageBounds:
       if ((s = refuse_overlaps(plan, inputs, outputs, "PageBounds")) != HYLE_HIP_OK) return s;
       err = launch_page_bounds(plan->page_bounds, inputs[0], static_cast<const int32_t *>(inputs[1]), static_cast<const int32_t *>(inputs[2]),
-                               outputs[0], aligned(inputs[0], 16) && aligned(outputs[0], 16), stream);
+                               outputs[0], stream);
       break;
     case Route::kPagedSelect:
       if ((s = refuse_overlaps(plan, inputs, outputs, "PagedSelect")) != HYLE_HIP_OK) return s;

@@ -340,8 +340,11 @@ def test_rotary_append_is_rope_and_paged_append():
 # ---- PageBounds ------------------------------------------------------------------------------
 @pytest.mark.parametrize("cache_tag", ["bf16", "f16", "f32", "e4m3", "mx4"])
 @pytest.mark.parametrize("depth,heads,page,newest,off", [(128, 8, 16, 1, 0), (64, 3, 1, 0, 0), (96, 2, 24, 30, 0), (256, 1, 256, 0, 0), (32, 5, 7, 4, 0),
-                                                         (128, 2, 64, 0, 4), (64, 2, 16, 0, 2), (320, 2, 16, 500, 0)])
+                                                         (128, 2, 64, 0, 4), (64, 2, 16, 0, 2), (320, 2, 16, 500, 0),
+                                                         (64, 1, 1100, 0, 0), (128, 2, 600, 700, 0), (160, 1, 288, 0, 0), (72, 3, 16, 2, 0), (256, 2, 8, 0, 0)])
 def test_bounds_of_pages(cache_tag, depth, heads, page, newest, off):
+    if cache_tag == "mx4" and depth % 32 != 0:
+        pytest.skip("4 bits come in blocks of 32")
     rng, lengths = np.random.default_rng(depth + page), (1, 300, page, 0, 3 * page + 1, -5)
     table, pages = pages_of(rng, lengths, page)
     table[1, 0] = (-1, pages, 2 ** 31 - 1)[heads % 3]
@@ -360,6 +363,8 @@ def test_bounds_of_pages(cache_tag, depth, heads, page, newest, off):
         if cache_tag == "f32":
             flat[3::97] = 3.4e38
             flat[5::89] = -1e-40
+        if cache_tag == "bf16":  # (a signaling one)
+            cache.view(torch.int16).view(-1)[11::113] = 0x7F81
     cache[int(table[4, 0]), 0, 0].view(torch.uint8)[...] = 255  # channels without a number (of e4m3, f16, bf16, f32 and 4 bits)
     before = rng.integers(0, 2 ** 15, (pages, 2, heads, depth)).astype(np.uint16)
     bounds = device(before.view(np.int16)).view(torch.bfloat16)
