@@ -447,7 +447,7 @@ struct RotaryAppendParams {
   Divisor page;
 };
 hipError_t launch_rotary_append(Elem type, const RotaryAppendParams &p, const void *projected, const void *positions, const void *frequencies,
-                                const int32_t *slots, void *cache, void *rotated, bool vector_aligned, hipStream_t stream);
+                                const int32_t *slots, void *cache, void *rotated, bool vector_aligned, int compute_units, hipStream_t stream);
 
 // PageBounds: the least and largest key of every channel of the pages that hold each sequence's newest tokens (0: any), outward to bf16.
 struct PageBoundsParams {

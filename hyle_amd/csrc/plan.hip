@@ -2352,7 +2352,7 @@ hyle_hip_status hyle_hip_plan_launch(const hyle_hip_plan *plan, const void *cons
       if ((s = refuse_overlaps(plan, inputs, outputs, "RotaryAppend")) != HYLE_HIP_OK) return s;
       err = launch_rotary_append(plan->elem, plan->rotary_append, inputs[0], inputs[1], inputs[2], static_cast<const int32_t *>(inputs[3]),
                                  outputs[0], output_count > 1 ? outputs[1] : nullptr,
-                                 aligned(inputs[0], 16) && aligned(outputs[0], 16) && (output_count < 2 || aligned(outputs[1], 16)), stream);
+                                 aligned(inputs[0], 16) && (output_count < 2 || aligned(outputs[1], 16)), (int)plan->context->compute_units, stream);
       break;
     case Route::kPageBounds:
       if ((s = refuse_overlaps(plan, inputs, outputs, "PageBounds")) != HYLE_HIP_OK) return s;

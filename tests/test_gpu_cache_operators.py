@@ -249,6 +249,12 @@ ROTARIES = [
     ("bf16", "bf16", 4, 2, 128, 2, PAIRS, 16, 65, False, False, 0),
     ("f16", "f16", 4, 2, 128, 120, PAIRS, 16, 65, False, False, 0),
     ("bf16", "mx4", 4, 2, 128, 120, HALF, 16, 65, False, False, 0),
+    ("bf16", "bf16", 7, 3, 128, 64, HALF, 16, 1, False, False, 0), ("f16", "f16", 6, 2, 80, 80, PAIRS, 16, 333, False, True, 0),
+    ("f16", "e4m3", 6, 2, 96, 48, HALF, 16, 333, True, False, 0), ("bf16", "e4m3", 5, 1, 256, 16, PAIRS, 8, 70, False, False, 0),
+    ("bf16", "mx4", 32, 8, 128, 128, HALF, 16, 64, False, False, 0), ("f16", "mx4", 3, 3, 32, 32, HALF, 16, 4500, False, False, 0),
+    ("bf16", "mx4", 2, 1, 992, 960, PAIRS, 4, 5, False, False, 0), ("f32", "f32", 4, 2, 64, 32, HALF, 16, 40, False, False, 0),
+    ("f32", "e4m3", 4, 2, 64, 64, PAIRS, 16, 40, False, False, 0), ("bf16", "bf16", 2, 1, 16, 16, HALF, 16, 5000, False, False, 0),
+    ("bf16", "mx4", 6, 2, 64, 64, HALF, 1, 40, False, False, 0), ("bf16", "mx4", 6, 2, 64, 64, HALF, 16, 40, False, False, 4),
 ]
 
 
