@@ -1,5 +1,5 @@
 // attention_split.hip -- attention of a few query rows over many keys, split over the keys and joined: f16 / bf16 queries,
-// keys and values of their type or e4m3, in memory or in a paged cache.
+// keys and values of their type or e4m3, in memory or in a paged cache, there also in 4 bits.
 //
 // Bound by the bytes of keys and values, which are read once for all rows of a key head (its query heads times the new
 // tokens).  The keys of all sequences, in tiles of 128, are dealt to a fixed number of chunks, however long each sequence is: a
@@ -13,6 +13,12 @@
 // non-temporal loads fast (64 sequences of 30 to 16384 keys, 8 key heads of 128, bf16, 760 MB: 130 us, 5.8 TB/s of the 7.0 that a
 // large read reaches; loads of 64 bytes of a row 200, by plain loads 150; 16 of 20000 to 32768 in e4m3, 852 MB: 146 us, 5.85 TB/s).
 // The next tile's keys are asked for when this one's are in LDS, its values likewise, the page numbers of the one after it too.
+// A cache in 4 bits is a quarter of the bytes for the same products, and there the waves' own work bounds a tile: codes to LDS, four
+// conversions to eight keys' elements, products, maximum, powers, values widened to LDS, products (64 sequences of 30 to 16384 keys, 8 key
+// heads of 128, 203 MB: 57.8 us, 3.5 TB/s; 51 with all pages one and the same, the vector unit busy for half of that, 57 with two
+// blocks to a unit instead of three, 121 with four, which spill; keys widened on the way to LDS instead of behind it 62.7).  The matrix unit's
+// own products with 4-bit numbers and their scales were tried with the queries as three rows of e4m3: it drops what is below 2^-12 of
+// the largest term, so logarithms of sums were off by 1.7e-4.
 // The waves' (m, l, O) are joined in LDS; a sequence of one chunk is then done, others leave theirs in the workspace for the
 // second kernel.
 #include "attention_math.h"
@@ -55,8 +61,10 @@ __device__ __forceinline__ uint32_t scanned(uint32_t v, int lane) {
 // The sequence and chunk that a slot of the grid is; false past the last.  Every wave of a launch comes to the same answer
 // from the marks alone.  target, chunks that all tiles are dealt to, is 0 where every sequence is one.  A block of one tile has
 // nothing to load while it computes, so a chunk has two at least where the tiles are more than the resident blocks (one sequence
-// of 32751 keys, 2 key heads of 256: 24 us with chunks of two tiles, 34 with one, 26 with four).
-__device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t *marks, int slot, int target, int blocks, SplitChunk *c) {
+// of 32751 keys, 2 key heads of 256: 24 us with chunks of two tiles, 34 with one, 26 with four).  Tiles of 4 bits are a quarter of the
+// bytes, so a block's start and end weigh more: there up to `least` = four where all chunks are then resident at once (one of 131055 keys: 38
+// us instead of 51).
+__device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t *marks, int slot, int target, int blocks, int least, SplitChunk *c) {
   const int lane = (int)threadIdx.x % kWaveLanes;
   if (target == 0) {
     if (slot >= p.sequences) return false;
@@ -65,7 +73,7 @@ __device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t
   }
   if (p.sequences == 1) {
     const int mark = __builtin_amdgcn_readfirstlane(attention_mark(p, marks, 0)), tiles = tiles_of(p, attention_sequence_of(p, 0, mark)).tiles;
-    const int each = max((int)(((uint32_t)tiles + (uint32_t)target - 1) / (uint32_t)target), tiles > blocks ? 2 : 1);
+    const int each = max((int)(((uint32_t)tiles + (uint32_t)target - 1) / (uint32_t)target), max(1, min(least, (int)(((uint32_t)tiles + (uint32_t)blocks - 1) / (uint32_t)blocks))));
     *c = SplitChunk{0, slot, max(1, (tiles + each - 1) / each), 0, each, mark};
     return slot < c->chunks;
   }
@@ -78,7 +86,7 @@ __device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t
     total += (uint32_t)__builtin_amdgcn_readlane((int)scanned(tiles_at(index, attention_mark(p, marks, min(index, p.sequences - 1))), lane), kWaveLanes - 1);
   }
   // (never more than a sequence can have)
-  const int each = (int)min(max((total + (uint32_t)target - 1) / (uint32_t)target, total > (uint32_t)blocks ? 2ull : 1ull), 1ull << 24);
+  const int each = (int)min(max((total + (uint32_t)target - 1) / (uint32_t)target, max((uint64_t)1, min((uint64_t)least, (total + (uint32_t)blocks - 1) / (uint32_t)blocks))), (uint64_t)1 << 24);
   int before = 0;
   for (int base = 0; base < p.sequences; base += kWaveLanes) {
     const int index = base + lane, mark = base == 0 ? first_mark : attention_mark(p, marks, min(index, p.sequences - 1));
@@ -178,6 +186,7 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
   constexpr int kVectors = kDepth / kLoad;               // of a row
   constexpr int kLoads = kStep * kVectors / kWaveLanes;  // of a lane, for a step's keys or values
   constexpr int kRow = kDepth * 2 + 32;                  // bytes of a row in LDS: 8 rows of 32 bytes fill the banks
+  constexpr int kCodeRow = kDepth / 2 + 16;              // of a row of codes; the step's scales, a word each, stand behind them
   constexpr int kJoinRow = kDepth + 4;                   // floats
   constexpr int kGroups = kWaves / kRowWaves;            // of waves that have keys of their own
   constexpr int kHeld = (kRowWaves == 1 ? 1 : 2) * kWaves * kStep * kRow, kJoined = kWaves * 16 * kJoinRow * 4;
@@ -189,7 +198,7 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
   const int slot = (int)layout.lanes.quotient(blockIdx.x), rest = (int)blockIdx.x - slot * (int)layout.lanes.divisor;
   const int group = (int)layout.row_tiles.quotient((uint32_t)rest), row_tile = rest - group * (int)layout.row_tiles.divisor;
   SplitChunk chunk;
-  if (!chunk_of(p, b.marks, slot, layout.target, layout.blocks, &chunk)) return;
+  if (!chunk_of(p, b.marks, slot, layout.target, layout.blocks, kFour ? 4 : 2, &chunk)) return;
   if (layout.target != 0 && chunk.chunk == 0 && rest == 0 && threadIdx.x == 0) layout.places[chunk.index] = int2{chunk.first_slot, chunk.chunks};
   const AttentionSequence s = attention_sequence_of(p, chunk.index, chunk.mark);
   const SplitTiles tiles = tiles_of(p, s);
@@ -213,61 +222,104 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
 
   const unsigned char *keys = static_cast<const unsigned char *>(b.key) + (int64_t)(group + s.head) * p.k_head;
   const unsigned char *values = static_cast<const unsigned char *>(b.value) + (int64_t)(group + s.head) * p.v_head;
-  const bool paged = p.kind == AttentionKind::kPaged;
+  const bool paged = kFour || p.kind == AttentionKind::kPaged;
   const int32_t *table = paged ? b.table + (int64_t)chunk.index * p.table_row : nullptr;
   auto first_of = [&](int tile) { return tile < tiles.sinks ? tile * kTile : tiles.low + (tile - tiles.sinks) * kTile; };
   auto first_key = [&](int tile) { return first_of(tile) + wave * kStep; };  // of the wave's own keys
   // A lane's key of a step, and the page that holds it; past the last key the last one's place is asked for.
-  auto page_of = [&](int tile) {
-    return paged ? table[p.page.quotient((uint32_t)min(first_key(tile) + lane % kStep, any.high - 1))] : 0;
+  // (4 bits: the lane's own rows of the loads)
+  constexpr int kPlaces = kFour ? kLoads : 1;
+  auto row_of = [&](int k) { return kFour ? k * (kWaveLanes / kVectors) + lane / kVectors : lane % kStep; };
+  int page[kPlaces];
+  // (Of 4 bits what lies behind the chunk's last tile is asked for too, all of it at one place: a load that is sometimes left out makes every
+  // wait for those before it one for all.  Of wider caches the loads themselves bound a tile, and short chunks would be 7 % slower.)
+  auto ask_pages = [&](int tile) {
+    if (kFour) tile = min(tile, end - 1);
+#pragma unroll
+    for (int k = 0; k < kPlaces; ++k) page[k] = paged ? table[p.page.quotient((uint32_t)min(first_key(tile) + row_of(k), any.high - 1))] : 0;
   };
   // One step's keys and values, whole rows side by side: a load's 64 vectors are whole cache lines, which non-temporal loads
   // need.  The next keys are asked for once these are in LDS, and so are the values.
   u32x4 key_words[kLoads], value_words[kLoads];
-  uint32_t key_scales[kFour ? kLoads : 1], value_scales[kFour ? kLoads : 1];  // bytes
+  uint32_t key_scales[kFour ? kLoads : 1], value_scales[kFour ? kLoads : 1];  // words that hold them
   uint32_t alive = 0;  // bit j: key j of the step is there and some row sees it
-  int64_t value_at = 0;
-  int scales_at = 0;  // from the codes of a row to its scales
+  int64_t value_at[kPlaces] = {};
+  int scales_at[kPlaces] = {};  // from the codes of a row to its scales
   const int vectors = p.depth / kLoad;  // of a row; zeros past them
   const int vector = lane % kVectors;
-  auto fetch = [&](const unsigned char *from, int64_t place, u32x4 (&words)[kLoads], uint32_t *scales) {
+  constexpr bool kEvenScales = kWhole && kDepth >= 128;  // a row's scales are whole words
+  uint32_t key_shifts[kPlaces], value_shifts[kPlaces];
+  auto scale_of = [&](uint32_t word, uint32_t shift) { return (word >> (kEvenScales ? (uint32_t)(vector % 4) * 8 : shift)) & 255u; };
+  auto fetch = [&](const unsigned char *from, const int64_t (&places)[kPlaces], u32x4 (&words)[kLoads], uint32_t *scales, uint32_t (&shifts)[kPlaces]) {
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
-      const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
-      const int64_t at = ((int64_t)__shfl((int)(place >> 32), row, kWaveLanes) << 32) | (uint32_t)__shfl((int)place, row, kWaveLanes);
       if (!kWhole) words[k] = u32x4{0, 0, 0, 0};
       if constexpr (kFour) {
-        const int there = __shfl(scales_at, row, kWaveLanes);
         if (!kWhole) scales[k] = 0;
         if (kWhole || vector < vectors) {
-          words[k] = load16_words(from + at, vector);
-          scales[k] = from[at + there + vector];
+          words[k] = load16_words(from + places[k], vector);
+          // (the word that holds the byte: a byte that is carried round the loop is widened, and so waited for, where it was loaded)
+          const unsigned char *byte = from + places[k] + scales_at[k] + vector;
+          if (!kEvenScales) shifts[k] = ((uint32_t)reinterpret_cast<uintptr_t>(byte) & 3u) * 8;
+          scales[k] = *reinterpret_cast<const uint32_t *>(byte - (kEvenScales ? vector % 4 : (int)(reinterpret_cast<uintptr_t>(byte) & 3u)));
         }
       } else {
+        const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
+        const int64_t at = ((int64_t)__shfl((int)(places[0] >> 32), row, kWaveLanes) << 32) | (uint32_t)__shfl((int)places[0], row, kWaveLanes);
         if (kWhole || vector < vectors) words[k] = load16_stream(from + at, vector);
       }
     }
   };
-  auto fetch_keys = [&](int tile, int page) {
-    const int key = first_key(tile) + lane % kStep, known = min(key, any.high - 1);
-    bool there = attention_sees(p, any, key) && (tile >= tiles.sinks || key < tiles.low);
-    int64_t key_at;
-    if (paged) {
-      there = there && (uint32_t)page < (uint32_t)p.pages;
-      const uint32_t at = (uint32_t)known - p.page.quotient((uint32_t)known) * p.page.divisor;
-      // (a page that is not there is read as the cache's first row, which is there: its keys are not alive)
-      key_at = value_at = there ? (int64_t)page * p.k_sequence + (int64_t)at * p.k_row : 0;
-      if constexpr (kFour) scales_at = (int)p.scale_offset - (there ? (int)at * ((int)p.k_row / 16 * 15) : 0);
-    } else {
-      key_at = (int64_t)chunk.index * p.k_sequence + (int64_t)known * p.k_row;
-      value_at = (int64_t)chunk.index * p.v_sequence + (int64_t)known * p.v_row;
+  auto fetch_keys = [&](int tile) {
+    int64_t key_at[kPlaces];
+    uint64_t lanes[kPlaces];  // whose key is there
+#pragma unroll
+    for (int k = 0; k < kPlaces; ++k) {
+      const int key = first_key(tile) + row_of(k), known = !kFour || tile < end ? min(key, any.high - 1) : 0;
+      bool there = (key < any.high) & ((key >= any.low) | (key < p.sinks)) & ((tile >= tiles.sinks) | (key < tiles.low)) & (!kFour || tile < end);
+      if (paged) {
+        there &= (uint32_t)page[k] < (uint32_t)p.pages;
+        const uint32_t at = (uint32_t)known - p.page.quotient((uint32_t)known) * p.page.divisor;
+        // (a page that is not there is read as the cache's first row, which is there: its keys are not alive)
+        key_at[k] = value_at[k] = there ? (int64_t)page[k] * p.k_sequence + (int64_t)at * p.k_row : 0;
+        if constexpr (kFour) scales_at[k] = (int)p.scale_offset - (there ? (int)at * ((int)p.k_row / 16 * 15) : 0);
+      } else {
+        key_at[k] = (int64_t)chunk.index * p.k_sequence + (int64_t)known * p.k_row;
+        value_at[k] = (int64_t)chunk.index * p.v_sequence + (int64_t)known * p.v_row;
+      }
+      lanes[k] = __ballot(there);
     }
-    alive = (uint32_t)__ballot(there);
-    fetch(keys, key_at, key_words, key_scales);
+    if constexpr (kFour) {
+      uint64_t all = lanes[0];
+#pragma unroll
+      for (int k = 1; k < kPlaces; ++k) all &= lanes[k];
+      alive = 0xFFFFFFFFu;
+      if (all != ~0ull) {
+        alive = 0;
+#pragma unroll
+        for (int k = 0; k < kPlaces; ++k)
+#pragma unroll 1
+          for (int r = 0; r < kWaveLanes / kVectors; ++r) alive |= (uint32_t)((lanes[k] >> (r * kVectors)) & 1) << (k * (kWaveLanes / kVectors) + r);
+      }
+    } else {
+      alive = (uint32_t)lanes[0];
+    }
+    fetch(keys, key_at, key_words, key_scales, key_shifts);
   };
-  auto fetch_values = [&]() { fetch(values, value_at, value_words, value_scales); };
+  auto fetch_values = [&]() { fetch(values, value_at, value_words, value_scales, value_shifts); };
+  // Rows widened from 4 bits are written by lanes whose pieces begin 64 bytes apart: eights of dims change places (by the turn of 64 dims
+  // that they are in, of depth 64 of the row), so that a write's pieces of 16 bytes, and a read's, lie in all banks.
+  auto swizzled = [](int row, int eight) { return kFour ? eight ^ (kDepth == 64 ? row / 2 % 2 : eight / 8 % 4) : eight; };
+  int put_at[4] = {}, read_at[2] = {};  // where a lane's four pieces go, and where it reads eights of even and odd turns
+  if constexpr (kFour) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) put_at[w] = lane / kVectors * kRow + 16 * swizzled(lane / kVectors, 4 * vector + w);
+    const int row = 4 * quarter + column / 4, eight = column % 4 / 2;  // (16 rows on, the same places)
+#pragma unroll
+    for (int turn = 0; turn < 2; ++turn) read_at[turn] = row * kRow + 16 * (eight ^ (kDepth == 64 ? row / 2 % 2 : turn)) + column % 2 * 8;
+  }
   // a step's vectors to the wave's rows in LDS, e4m3 and 4 bits as the elements of T that they stand for (kClean: numbers alone)
-  auto put = [&](unsigned char *base, const u32x4 (&words)[kLoads], const uint32_t *scales, auto clean) {
+  auto put = [&](unsigned char *base, const u32x4 (&words)[kLoads], const uint32_t *scales, const uint32_t (&shifts)[kPlaces], auto clean) {
     constexpr bool kClean = decltype(clean)::value;
     __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses are in order)
 #pragma unroll
@@ -277,9 +329,9 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
       if constexpr (kFour) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          u32x4 wide = widened4<T>(words[k][w], bits_f32(scales[k] << 23));
+          u32x4 wide = widened4<T>(words[k][w], bits_f32(scale_of(scales[k], shifts[kFour ? k : 0]) << 23));
           if (kClean) wide = numbers_only<T>(wide);
-          *reinterpret_cast<u32x4 *>(to + 16 * w) = wide;
+          *reinterpret_cast<u32x4 *>(base + put_at[w] + k * (kWaveLanes / kVectors) * kRow) = wide;
         }
       } else if constexpr (kNarrow) {
         u32x4 low, high;
@@ -293,11 +345,23 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
     __builtin_amdgcn_wave_barrier();  // other lanes' rows are read next
   };
 
+  // Keys in 4 bits go to LDS as they are and are widened where they are multiplied: a lane then has kDepth / 4 neighbouring dims of its
+  // key, and its queries' in the same order.
+  auto put_codes = [&](unsigned char *base) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const int row = k * (kWaveLanes / kVectors) + lane / kVectors;
+      *reinterpret_cast<u32x4 *>(base + row * kCodeRow + vector * 16) = key_words[k];
+      *reinterpret_cast<uint32_t *>(base + kStep * kCodeRow + (row * kVectors + vector) * 4) = scale_of(key_scales[k], key_shifts[k]) << 23;
+    }
+    __builtin_amdgcn_wave_barrier();
+  };
+  auto dims_of = [&](int k) { return kFour ? quarter * kSteps + k : 4 * k + quarter; };  // of a product, in eights
   auto key_rows = [&](int part) { return held + part * kStep * kRow; };
   auto value_rows = [&](int part) { return held + ((kRowWaves == 1 ? 0 : kWaves) + part) * kStep * kRow; };
-  int page = 0;
-  if (begin < end) page = page_of(begin);
-  // queries: a lane's row is its column, its dims 8 quarter on of every 32
+  if (begin < end) ask_pages(begin);
+  // queries: a lane's row is its column, its dims 8 quarter on of every 32 (with keys in 4 bits, a quarter of all in a row)
   u32x4 query[kSteps];
   AttentionSpan span;
   {
@@ -307,14 +371,20 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       query[k] = u32x4{0, 0, 0, 0};
-      if (row < layout.rows && (kWhole || (4 * k + quarter) * 8 < p.depth)) query[k] = load16(from, 4 * k + quarter);
+      if (row < layout.rows && (kWhole || dims_of(k) * 8 < p.depth)) query[k] = load16(from, dims_of(k));
     }
   }
   if (kRowWaves > 1 && threadIdx.x == 0) no_number = 0;
   if (begin < end) {
-    fetch_keys(begin, page);
+    fetch_keys(begin);
+    if constexpr (kFour) {
+      __builtin_amdgcn_sched_barrier(0);  // (in the loop's order: its waits count what was asked for since)
+      ask_pages(begin + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     fetch_values();
-    if (begin + 1 < end) page = page_of(begin + 1);
+    if (!kFour && begin + 1 < end) ask_pages(begin + 1);
+    if constexpr (kFour) __builtin_amdgcn_sched_barrier(0);
   }
   if (p.scale <= 0.0f) {
 #pragma unroll
@@ -347,7 +417,7 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
         float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float x = Traits<T>::load(from + j * kRow, 16 * d + 4 * quarter + r);
+          const float x = Traits<T>::load(from + j * kRow, 8 * swizzled(j, 2 * d + quarter / 2) + quarter % 2 * 4 + r);
           v[r] = fabsf(x) < INFINITY ? 0.0f : x;
         }
         if (sees) out[d] += f32x4{v[0], v[1], v[2], v[3]};
@@ -360,7 +430,7 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
       // (of 4 bits by the scale: from which on 6 of it, or 4, may pass T's range, and NaN)
-      if constexpr (kFour) found |= (uint32_t)(value_scales[k] >= (std::is_same<T, BF16>::value ? 253u : 141u));
+      if constexpr (kFour) found |= (uint32_t)(scale_of(value_scales[k], value_shifts[k]) >= (std::is_same<T, BF16>::value ? 253u : 141u));
       else found |= no_numbers<C>(value_words[k]);
     }
     return __ballot(found != 0) != 0;
@@ -376,19 +446,20 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
 
   for (int tile = begin; tile < end; ++tile) {
     const uint32_t own = alive;
-    put(key_rows(wave), key_words, key_scales, kAsRead);
+    if constexpr (kFour) put_codes(key_rows(wave));
+    else put(key_rows(wave), key_words, key_scales, key_shifts, kAsRead);
     if constexpr (kRowWaves == 1) {
       __builtin_amdgcn_sched_barrier(0);  // (loads that move up further need registers of their own)
-      if (tile + 1 < end) {
-        fetch_keys(tile + 1, page);
-        if (tile + 2 < end) page = page_of(tile + 2);
+      if (kFour || tile + 1 < end) {
+        fetch_keys(tile + 1);
+        if (kFour || tile + 2 < end) ask_pages(tile + 2);
       }
     } else {
       clear_dead(own);
       if (lane == 0) shared_alive[wave] = own;
       const bool odd = s.rows > 1 && !(own == 0xFFFFFFFFu && seen_whole(first_key(tile))) && any_no_number();
       if (odd && lane == 0) no_number = tile + 1;
-      put(value_rows(wave), value_words, value_scales, kAsRead);
+      put(value_rows(wave), value_words, value_scales, value_shifts, kAsRead);
       __syncthreads();
       if (no_number == tile + 1) {
 #pragma unroll 1
@@ -398,13 +469,13 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
         }
         __syncthreads();
         keep_numbers();
-        put(value_rows(wave), value_words, value_scales, kNumbers);
+        put(value_rows(wave), value_words, value_scales, value_shifts, kNumbers);
         __syncthreads();
       }
       __builtin_amdgcn_sched_barrier(0);
       if (tile + 1 < end) {
-        fetch_keys(tile + 1, page);
-        if (tile + 2 < end) page = page_of(tile + 2);
+        fetch_keys(tile + 1);
+        if (tile + 2 < end) ask_pages(tile + 2);
         fetch_values();
       }
     }
@@ -418,10 +489,29 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         score[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (kFour) {
+          const unsigned char *codes = from + (16 * half + column) * kCodeRow + quarter * (kSteps * 4);
+          const unsigned char *scales = from + kStep * kCodeRow + (16 * half + column) * kVectors * 4 + quarter * kSteps / 4 * 4;
+          uint32_t words[kSteps];
+          if constexpr (kSteps == 2) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(codes);
+            words[0] = w.x, words[1] = w.y;
+          } else {
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          const u32x4 w = *reinterpret_cast<const u32x4 *>(from + (16 * half + column) * kRow + (4 * k + quarter) * 16);
-          score[half] = product16<T>(w, query[k], score[half]);
+            for (int v = 0; v < kSteps / 4; ++v) {
+              const u32x4 w = reinterpret_cast<const u32x4 *>(codes)[v];
+              words[4 * v] = w.x, words[4 * v + 1] = w.y, words[4 * v + 2] = w.z, words[4 * v + 3] = w.w;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k)
+            score[half] = product16<T>(widened4<T>(words[k], reinterpret_cast<const float *>(scales)[k / 4]), query[k], score[half]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(from + (16 * half + column) * kRow + (4 * k + quarter) * 16);
+            score[half] = product16<T>(w, query[k], score[half]);
+          }
         }
       }
       if (!whole) {
@@ -461,19 +551,21 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
         clear_dead(these);
         const bool odd = !whole && s.rows > 1 && any_no_number();
         if (odd) {
-          put(value_rows(wave), value_words, value_scales, kAsRead);
+          put(value_rows(wave), value_words, value_scales, value_shifts, kAsRead);
           add_no_numbers(value_rows(wave), these, first);
           keep_numbers();
         }
-        if (kFour && odd) put(value_rows(wave), value_words, value_scales, kNumbers);
-        else put(value_rows(wave), value_words, value_scales, kAsRead);
+        put(value_rows(wave), value_words, value_scales, value_shifts, kAsRead);
+        if (kFour && odd) put(value_rows(wave), value_words, value_scales, value_shifts, kNumbers);
         __builtin_amdgcn_sched_barrier(0);
-        if (tile + 1 < end) fetch_values();
+        if (kFour || tile + 1 < end) fetch_values();
+        if constexpr (kFour) __builtin_amdgcn_sched_barrier(0);
       }
       from = value_rows(part);
 #pragma unroll
       for (int d = 0; d < kDims; ++d) {
-        const unsigned char *at = from + (4 * quarter + column / 4) * kRow + (d * 16 + column % 4 * 4) * 2;
+        const unsigned char *at = kFour ? from + read_at[kDepth == 64 ? 0 : d / 4 % 2] + 32 * (d ^ (kDepth == 64 ? 0 : d / 8 % 2))
+                                        : from + (4 * quarter + column / 4) * kRow + (d * 16 + column % 4 * 4) * 2;
         const uint2 near = read_transposed(at), far = read_transposed(at + 16 * kRow);
         const u32x4 value = {near.x, near.y, far.x, far.y};
         out[d] = product16<T>(value, weights, out[d]);

@@ -150,6 +150,7 @@ DECODES_4 = [
     ("bf16", 32, 14, 2, 16, (140, 1000), 8, 0, 0, False, 0), ("f16", 64, 24, 1, 16, (140, 1000), 1, 0, 0, True, 0),
     ("bf16", 96, 24, 2, 8, (140, 3, 1000), 2, 0, 0, True, 0), ("f16", 96, 40, 1, 8, (140, 1000), 1, 0, 0, False, 0),
     ("f16", 128, 8, 1, 4, (5, 1000), 4, 64, 0, True, 0), ("bf16", 224, 4, 2, 16, (900, 70), 1, 0, 0, True, 0),
+    ("bf16", 128, 8, 2, 16, (0, -3, 0), 1, 0, 0, True, 0), ("f16", 64, 8, 2, 16, (0,), 2, 0, 0, True, 0),
     ("f16", 192, 20, 1, 16, (900, 70), 3, 0, 0, False, 0), ("bf16", 256, 8, 1, 16, (900, 70, 2), 3, 0, 0, True, 0),
 ]
 
@@ -157,7 +158,7 @@ DECODES_4 = [
 @pytest.mark.parametrize("tag,depth,queries,heads,page,lengths,new,window,sinks,logs,off", DECODES_4)
 def test_attention_over_four_bits(tag, depth, queries, heads, page, lengths, new, window, sinks, logs, off):
     rng = np.random.default_rng(depth + queries)
-    table, pages = pages_of(rng, lengths, page)
+    table, pages = pages_of(rng, lengths, page, columns=max(40, -(-max(lengths) // page)))
     cache = cache_of(rng, pages, heads, page, depth, "mx4")
     cache = off_by(cache, off) if off else cache
     query = values(rng, (len(lengths), new, queries, depth), tag, 0.7)
@@ -166,9 +167,9 @@ def test_attention_over_four_bits(tag, depth, queries, heads, page, lengths, new
     outputs = submit(operation, [query, cache, device(table), torch.tensor(lengths, dtype=torch.int32, device=DEVICE)])
     held = cs.cache_values(cache)
     for i, n in enumerate(lengths):
-        place = np.arange(n)
+        place = np.arange(max(n, 0))
         k, v = (held[table[i, place // page], side, :, place % page] for side in (0, 1))
-        want, want_logs, bound, log_bound = attention_rows(host(query[i]), k, v, n - new, True, window, sinks, operation.scale, query.dtype)
+        want, want_logs, bound, log_bound = attention_rows(host(query[i]), k, v, max(n, 0) - new, True, window, sinks, operation.scale, query.dtype)
         assert_within(outputs[0][i], want, bound)
         if logs:
             assert_within(outputs[1][i], want_logs, log_bound)
