@@ -231,10 +231,12 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
   constexpr int kPlaces = kFour ? kLoads : 1;
   auto row_of = [&](int k) { return kFour ? k * (kWaveLanes / kVectors) + lane / kVectors : lane % kStep; };
   int page[kPlaces];
-  // (Of 4 bits what lies behind the chunk's last tile is asked for too, all of it at one place: a load that is sometimes left out makes every
-  // wait for those before it one for all.  Of wider caches the loads themselves bound a tile, and short chunks would be 7 % slower.)
+  // What lies behind the chunk's last tile is asked for too, all of it at one place: a load that is sometimes left out makes every wait for
+  // those before it one for all.  It pays where a block has its unit almost to itself and a cache in 4 bits (one of 131055 keys: 34.6 us
+  // without, 30.3 so; of depth 128 two tiles to a chunk 8.8 without, 10.7 so, many the same).
+  constexpr bool kPast = kFour && kDepth == 256;
   auto ask_pages = [&](int tile) {
-    if (kFour) tile = min(tile, end - 1);
+    if (kPast) tile = min(tile, end - 1);
 #pragma unroll
     for (int k = 0; k < kPlaces; ++k) page[k] = paged ? table[p.page.quotient((uint32_t)min(first_key(tile) + row_of(k), any.high - 1))] : 0;
   };
@@ -450,9 +452,9 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
     else put(key_rows(wave), key_words, key_scales, key_shifts, kAsRead);
     if constexpr (kRowWaves == 1) {
       __builtin_amdgcn_sched_barrier(0);  // (loads that move up further need registers of their own)
-      if (kFour || tile + 1 < end) {
+      if (kPast || tile + 1 < end) {
         fetch_keys(tile + 1);
-        if (kFour || tile + 2 < end) ask_pages(tile + 2);
+        if (kPast || tile + 2 < end) ask_pages(tile + 2);
       }
     } else {
       clear_dead(own);
@@ -558,7 +560,7 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
         put(value_rows(wave), value_words, value_scales, value_shifts, kAsRead);
         if (kFour && odd) put(value_rows(wave), value_words, value_scales, value_shifts, kNumbers);
         __builtin_amdgcn_sched_barrier(0);
-        if (kFour || tile + 1 < end) fetch_values();
+        if (kPast || tile + 1 < end) fetch_values();
         if constexpr (kFour) __builtin_amdgcn_sched_barrier(0);
       }
       from = value_rows(part);
