@@ -62,8 +62,8 @@ __device__ __forceinline__ uint32_t scanned(uint32_t v, int lane) {
 // from the marks alone.  target, chunks that all tiles are dealt to, is 0 where every sequence is one.  A block of one tile has
 // nothing to load while it computes, so a chunk has two at least where the tiles are more than the resident blocks (one sequence
 // of 32751 keys, 2 key heads of 256: 24 us with chunks of two tiles, 34 with one, 26 with four).  Tiles of 4 bits are a quarter of the
-// bytes, so a block's start and end weigh more: there up to `least` = four where all chunks are then resident at once (one of 131055 keys: 38
-// us instead of 51).
+// bytes, so a block's start and end weigh more, and key heads with pages of their own are many short sequences alike: there up to `least` = four,
+// where all chunks are then resident at once (one of 131055 keys: 38 us instead of 51; 128 key heads of 2048 keys in bf16 28.6 instead of 31).
 __device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t *marks, int slot, int target, int blocks, int least, SplitChunk *c) {
   const int lane = (int)threadIdx.x % kWaveLanes;
   if (target == 0) {
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
   const int slot = (int)layout.lanes.quotient(blockIdx.x), rest = (int)blockIdx.x - slot * (int)layout.lanes.divisor;
   const int group = (int)layout.row_tiles.quotient((uint32_t)rest), row_tile = rest - group * (int)layout.row_tiles.divisor;
   SplitChunk chunk;
-  if (!chunk_of(p, b.marks, slot, layout.target, layout.blocks, kFour ? 4 : 2, &chunk)) return;
+  if (!chunk_of(p, b.marks, slot, layout.target, layout.blocks, kFour || p.apart.divisor != 1 ? 4 : 2, &chunk)) return;
   if (layout.target != 0 && chunk.chunk == 0 && rest == 0 && threadIdx.x == 0) layout.places[chunk.index] = int2{chunk.first_slot, chunk.chunks};
   const AttentionSequence s = attention_sequence_of(p, chunk.index, chunk.mark);
   const SplitTiles tiles = tiles_of(p, s);
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
     for (int k = 0; k < kLoads; ++k) {
       if (!kWhole) words[k] = u32x4{0, 0, 0, 0};
       if constexpr (kFour) {
-        if (!kWhole) scales[k] = 0;
+        if (!kWhole) scales[k] = 0, shifts[k] = 0;
         if (kWhole || vector < vectors) {
           words[k] = load16_words(from + places[k], vector);
           // (the word that holds the byte: a byte that is carried round the loop is widened, and so waited for, where it was loaded)

@@ -421,6 +421,7 @@ SELECTS = [
     ("f16", 7, 1, 64, 16, 9, 1, (3000, 170), 0), ("bf16", 14, 2, 256, 16, 9, 1, (3000, 170), 0), ("f32", 12, 2, 128, 16, 9, 2, (3000, 170), 0),
     ("bf16", 6, 3, 64, 1, 700, 2, (30011, 29000), 0), ("f16", 5, 1, 128, 1, 30, 3, (40001,), 0), ("bf16", 4, 2, 256, 1, 3000, 1, (9000, 4099, 300), 0),
     ("f32", 2, 2, 136, 1, 5, 1, (16384, 16385), 0), ("f16", 4, 1, 96, 1, 16000, 1, (17000, 40000), 0),
+    ("bf16", 24, 2, 64, 16, 9, 1, (3000, 170), 0),
 ]
 
 
@@ -534,6 +535,34 @@ def test_steps_of_sparse_decoding(tag, cache_tag):
                 k, v = (held[want_pages[i, h, place // page], side, h, place % page][:, None] for side in (0, 1))
                 want, _, bound, _ = attention_rows(q[i:i + 1, mine], k, v, int(want_seen[i, h]) - 1, True, 0, 0, scale, TYPES[tag])
                 assert_within(out[i:i + 1, mine], want, bound)
+
+
+@pytest.mark.parametrize("cache_tag,pages", [("mx4", 300_000), ("bf16", 70_000)])
+def test_pages_beyond_32_bits(cache_tag, pages):
+    """The last pages of a cache of more than 4 GiB, and the same in a small one."""
+    rng, heads, queries, depth, page, tokens = np.random.default_rng(5), 8, 16, 128, 16, 200
+    projected = values(rng, (tokens, queries + 2 * heads, depth), "bf16")
+    positions, frequencies = torch.arange(tokens, dtype=torch.int32, device=DEVICE), device((10000.0 ** (-np.arange(64) / 64)).astype(np.float32))
+    answers = []
+    for count in (pages, 16):
+        row = depth // 32 * 17 if cache_tag == "mx4" else depth
+        cache = torch.zeros((count, 2, heads, page, row), dtype=TYPES[cache_tag], device=DEVICE)
+        assert count == 16 or cache.numel() * cache.element_size() > 2 ** 32
+        slots = torch.arange(count * page - tokens, count * page, dtype=torch.int32, device=DEVICE)
+        table = torch.arange(count - 13, count, dtype=torch.int32, device=DEVICE)[None].contiguous()  # 200 tokens end a page: 8 places of the first are free
+        note(f"pages beyond 32 bits {cache_tag} {count}")
+        _, rotated = submit(hc.RotaryAppend(count, page, tio.desc_of(cache).data_type, heads, HALF), [projected, positions, frequencies, slots], [cache])
+        lengths = torch.tensor([13 * page], dtype=torch.int32, device=DEVICE)
+        (bounds,) = submit(hc.PageBounds(), [cache, table, lengths], [torch.zeros((count, 2, heads, depth), dtype=torch.bfloat16, device=DEVICE)])
+        chosen, seen = submit(hc.PagedSelect(4, page), [rotated[-1:], bounds, table, lengths])
+        (out,) = submit(hc.PagedAttention(0.1), [rotated[-1:], cache, chosen, seen])
+        (whole,) = submit(hc.PagedAttention(0.1), [rotated[-1:], cache, table, lengths])
+        answers.append((cache[-13:].clone(), bounds[-13:].clone(), chosen - count, seen, out, whole))
+        del cache, bounds
+        torch.cuda.empty_cache()
+    for far, near in zip(*answers):
+        assert torch.equal(far, near)
+    assert (answers[0][4] != 0).any()
 
 
 def test_an_output_within_an_operand_is_refused():
