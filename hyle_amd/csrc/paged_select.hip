@@ -430,7 +430,8 @@ hipError_t launch_paged_select(Elem type, const PagedSelectParams &p, const void
                                int compute_units, hipStream_t stream) {
   const SelectBuffers b{static_cast<const unsigned char *>(query), static_cast<const unsigned char *>(bounds), table, lengths, static_cast<uint32_t *>(workspace)};
   if (p.columns > p.count) {
-    const bool vectors = vector_aligned && p.depth % 8 == 0 && (p.q_sequence | p.q_row | p.q_head | p.b_page | p.b_side | p.b_head) % 16 == 0;
+    // (lanes without a page read the first one's bounds, so there has to be one)
+    const bool vectors = vector_aligned && p.pages != 0 && p.depth % 8 == 0 && (p.q_sequence | p.q_row | p.q_head | p.b_page | p.b_side | p.b_head) % 16 == 0;
     switch (type) {
       case Elem::kF32: start_scores<F32>(p, b, vectors, compute_units, stream); break;
       case Elem::kF16: start_scores<F16>(p, b, vectors, compute_units, stream); break;

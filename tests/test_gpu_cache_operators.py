@@ -462,6 +462,18 @@ def test_choices_at_the_edges():
         assert np.array_equal(got[1].cpu().numpy(), want[1]), count
 
 
+def test_a_choice_where_no_page_has_bounds():
+    """A cache without pages: all scores are the least, so the earlier pages of the table are chosen."""
+    rng, lengths = np.random.default_rng(3), (700, 40)
+    table, _ = pages_of(rng, lengths, 16)
+    query = values(rng, (2, 1, 4, 64), "bf16")
+    bounds = torch.zeros((0, 2, 2, 64), dtype=torch.bfloat16, device=DEVICE)
+    note("select without pages")
+    got = submit(hc.PagedSelect(5, 16), [query, bounds, device(table), torch.tensor(lengths, dtype=torch.int32, device=DEVICE)])
+    want = cs.selected(host(query), np.zeros((0, 2, 2, 64)), table, lengths, 2, 16, 5)
+    assert np.array_equal(got[0].cpu().numpy(), want[0]) and np.array_equal(got[1].cpu().numpy(), want[1])
+
+
 # ---- together --------------------------------------------------------------------------------
 @pytest.mark.parametrize("tag,cache_tag", [("bf16", "bf16"), ("f16", "mx4"), ("bf16", "e4m3")])
 def test_steps_of_sparse_decoding(tag, cache_tag):
