@@ -1088,8 +1088,8 @@ hyle_hip_status admit_attention(hyle_hip_plan *p, uint32_t units) {
       return fail(HYLE_HIP_UNIMPLEMENTED, "paged attention requires pages and positions within int32");
     if (!has_whole_pages(cache)) return fail(HYLE_HIP_UNIMPLEMENTED, "a cache of 4 bits requires rows of a page behind one another");
     if (table.rank == 3) {
-      // each key head of a sequence is a sequence of the kernels
-      if (columns != 0 && ((heads > 1 && query.dims[0] > 1 && table.byte_strides[0] != heads * table.byte_strides[1]) || !is_dense(lengths)))
+      // each key head of a sequence is a sequence of the kernels (which read its length also where the table is empty)
+      if ((columns != 0 && heads > 1 && query.dims[0] > 1 && table.byte_strides[0] != heads * table.byte_strides[1]) || !is_dense(lengths))
         return fail(HYLE_HIP_UNIMPLEMENTED, "paged attention requires pages of key heads at one stride and dense lengths");
       a.sequences *= a.heads;
       a.apart = Divisor((uint32_t)heads);

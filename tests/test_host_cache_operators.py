@@ -164,3 +164,15 @@ def test_blocks_of_four_bits_by_hand():
     assert joined.shape == (3, 3, 17)
     again = cs.mx4_split(joined)
     assert np.array_equal(again[0], codes.reshape(3, 3, 16)) and np.array_equal(again[1], scales.reshape(3, 3, 1))
+
+
+@pytest.mark.parametrize("cache", [CACHE, FOUR])
+@pytest.mark.parametrize("strides", [(0, 4), (32, 4), (4, 8)])
+def test_lengths_of_key_heads_are_dense_also_where_the_table_is_empty(cache, strides):
+    """The kernels read a length of every sequence and key head, pages or not: those of one sequence for all would be read past their end."""
+    for columns in (3, 0):
+        table = D(I32, [2, 4, columns])
+        with pytest.raises(hc.StatusError) as refused:
+            hc.prepare(CTX, hc.PagedAttention(), Q, cache, table, _strided(I32, (2, 4), strides))
+        assert refused.value.code == hc.StatusCode.kUnimplemented, refused.value
+        assert hc.prepare(CTX, hc.PagedAttention(), Q, cache, table, D(I32, [2, 4])).dispatch_count() >= 1
