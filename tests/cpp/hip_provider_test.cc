@@ -805,6 +805,40 @@ DEVICE_TEST(RotaryAppendTurnsQueriesAndKeys) {
   EXPECT(got == std::vector<float>({1, 2, 3, 4, 1 * c - 2 * s, 1 * s + 2 * c, 3, 4}));
 }
 
+DEVICE_TEST(PagedSelectFindsThePageThatPageBoundsDescribes) {
+  // six keys of one head of four dims in pages of one: the query's products are largest in the page at place 3, and the first and the last are
+  // always chosen
+  const TensorDesc cache = dense(DataType::kFloat32, {7, 2, 1, 1, 4}), pages = dense(DataType::kInt32, {1, 6}), lengths = dense(DataType::kInt32, {1});
+  const TensorDesc bounds = dense(DataType::kBFloat16, {7, 2, 1, 4}), query = dense(DataType::kFloat32, {1, 1, 4});
+  auto bound = prepare(fixture().context, PageBounds{.newest = 0}, cache, pages, lengths);
+  auto choose = prepare(fixture().context, PagedSelect{.count = 3, .page_size = 1}, query, bounds, pages, lengths);
+  REQUIRE(bound.has_value() && choose.has_value());
+  EXPECT(choose->dispatch_count() == 2);
+  std::vector<float> held(7 * 2 * 4, 0.0F);
+  const std::int32_t order[6] = {6, 1, 0, 4, 2, 5};
+  for (int place = 0; place < 6; ++place) held[order[place] * 8] = static_cast<float>(place == 3 ? 2 : -place), held[order[place] * 8 + 1] = 1.0F;
+  DeviceBuffer keys = upload(held), table = upload(std::vector<std::int32_t>(order, order + 6)), length = upload(std::vector<std::int32_t>{6});
+  DeviceBuffer edges = upload(std::vector<std::uint16_t>(7 * 2 * 4, 7)), q = upload(std::vector<float>{1, 0.5F, 0, 0});
+  DeviceBuffer chosen = upload(std::vector<std::int32_t>(3, 9)), seen = upload(std::vector<std::int32_t>(1, 9));
+  DeviceBuffer workspace = DeviceBuffer::create(choose->workspace_requirement().size).value();
+  auto first = bound->create_invocation();
+  auto second = choose->create_invocation(workspace.data(), workspace.size());
+  REQUIRE(first.has_value() && second.has_value());
+  auto written = first->submit(fixture().queue, {*ConstTensorView::create(cache, keys), *ConstTensorView::create(pages, table),
+                                                 *ConstTensorView::create(lengths, length)}, {*TensorView::create(bounds, edges)});
+  REQUIRE(written.has_value());
+  auto read = second->submit(fixture().queue, {*ConstTensorView::create(query, q), *ConstTensorView::create(bounds, edges), *ConstTensorView::create(pages, table),
+                                               *ConstTensorView::create(lengths, length)},
+                             {*TensorView::create(dense(DataType::kInt32, {1, 1, 3}), chosen), *TensorView::create(dense(DataType::kInt32, {1, 1}), seen)});
+  REQUIRE(read.has_value());
+  EXPECT(read->wait().ok());
+  EXPECT(download<std::int32_t>(chosen, 3) == std::vector<std::int32_t>({6, 4, 5}));
+  EXPECT(download<std::int32_t>(seen, 1) == std::vector<std::int32_t>({3}));
+  const std::vector<std::uint16_t> kept = download<std::uint16_t>(edges, 7 * 2 * 4);
+  for (int side = 0; side < 2; ++side) EXPECT(kept[4 * 8 + side * 4] == 0x4000 && kept[4 * 8 + side * 4 + 1] == 0x3F80);  // a key is both of its page's bounds
+  for (int i = 0; i < 8; ++i) EXPECT(kept[3 * 8 + i] == 7);                                                              // a page of no sequence
+}
+
 DEVICE_TEST(RejectedSubmissionsEnqueueNothing) {
   const TensorDesc d = dense(DataType::kFloat32, {8, 64}), row = dense(DataType::kFloat32, {64});
   auto prepared = prepare(fixture().context, Binary{BinaryKind::kMultiply}, d, row);
