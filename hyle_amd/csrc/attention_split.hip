@@ -6,7 +6,9 @@
 // chunk is ceil(tiles / chunks) tiles of one sequence.  A block takes one chunk of one key head:
 //   S^T[key, row] = K Q^T,  p = 2^(S^T c - m),  O^T[dim, row] = V^T P^T   (c = scale * log2(e))
 // with the running maximum m and sum l of the softmax per lane (a lane's row is its column).  Weights are rounded once to the
-// queries' type, which the matrix unit asks for; sums, statistics and what chunks leave are f32.  Up to 16 rows, its four waves each
+// queries' type, which the matrix unit asks for (the mean distance of bf16 outputs from 64 bits, with weights in f32 / here: over 4 bits, one
+// sequence of 131055 keys, 3.2e-4 / 3.4e-4, over 2048 keys of each key head in bf16 7.3e-5 / 1.09e-4; the outputs' own rounding is most
+// of it); sums, statistics and what chunks leave are f32.  Up to 16 rows, its four waves each
 // take 32 keys of every tile and do not meet before the end; 32 or 64 rows are dealt to the waves, which share the tile's keys
 // in LDS (64 rows to every wave spilled: 93 sequences of 8 new tokens, 8 key heads of 128, 118 us, shared 68).  Keys go through LDS
 // too, not only the values that are read by columns: whole rows side by side are whole cache lines, and only of those are
@@ -63,7 +65,13 @@ __device__ __forceinline__ uint32_t scanned(uint32_t v, int lane) {
 // nothing to load while it computes, so a chunk has two at least where the tiles are more than the resident blocks (one sequence
 // of 32751 keys, 2 key heads of 256: 24 us with chunks of two tiles, 34 with one, 26 with four).  Tiles of 4 bits are a quarter of the
 // bytes, so a block's start and end weigh more, and key heads with pages of their own are many short sequences alike: there up to `least` = four,
-// where all chunks are then resident at once (one of 131055 keys: 38 us instead of 51; 128 key heads of 2048 keys in bf16 28.6 instead of 31).
+// where all chunks are then resident at once.  (us with two at least / up to four.  4 bits, depths 64, 128 and 256, bf16: one of 131055 keys 34.1 / 30.5,
+// 45.1 / 45.1, 50.5 / 37.5; 16 of 4000, 4 new tokens each 23.9 / 18.9, 36.4 / 32.5, 39.5 / 31.3; 8 of 3000 12.4 / 12.5, 14.5 / 14.7, 19.0 / 19.1; 64 ragged
+// ones 38.9 / 40.1, 57.8 / 57.7, 59.3 / 55.0; f16 alike.  128 key heads of 2048 keys of their own: bf16 17.8 / 17.8, 33.1 / 30.6, 66.2 / 62.1, e4m3
+// 15.6 / 15.6, 25.0 / 21.7, 40.3 / 35.6, 4 bits 14.6 / 14.7, 20.9 / 17.5, 44.5 / 35.2; 32 of them or fewer the same within 3 %.)
+// Every wave goes through all marks for its answer: little of a block's time for 64 sequences and a multiple of it for thousands, which pages of
+// key heads come to sooner (640 keys, 8 key heads of 128, bf16, pages of the sequences / of each key head: 64 sequences 39 / 58, 256 117 / 235,
+// 1024 523 / 1770; 2048 keys, 16 30 / 32, 64 92 / 107).
 __device__ __forceinline__ bool chunk_of(const AttentionParams &p, const int32_t *marks, int slot, int target, int blocks, int least, SplitChunk *c) {
   const int lane = (int)threadIdx.x % kWaveLanes;
   if (target == 0) {
@@ -138,7 +146,7 @@ template <class T> __device__ __forceinline__ void widened(u32x4 w, u32x4 *low, 
   *low = u32x4{a.x, a.y, b.x, b.y};
   *high = u32x4{c.x, c.y, d.x, d.y};
 }
-// 32 values in 4 bits as sixteen words of T by their scale: exact, but for f16's range.
+// Eight values in 4 bits as four words of T by their scale: exact, but for f16's range.
 template <class T> __device__ __forceinline__ u32x4 widened4(uint32_t w, float scale) {
   u32x4 out;
   if constexpr (std::is_same<T, BF16>::value) {
@@ -238,8 +246,10 @@ __global__ __launch_bounds__(kThreads, resident(!std::is_same<C, T>::value, kDep
   auto row_of = [&](int k) { return kFour ? k * (kWaveLanes / kVectors) + lane / kVectors : lane % kStep; };
   int page[kPlaces];
   // What lies behind the chunk's last tile is asked for too, all of it at one place: a load that is sometimes left out makes every wait for
-  // those before it one for all.  It pays where a block has its unit almost to itself and a cache in 4 bits (one of 131055 keys: 34.6 us
-  // without, 30.3 so; of depth 128 two tiles to a chunk 8.8 without, 10.7 so, many the same).
+  // those before it one for all.  It pays where a block has its unit almost to itself and a cache in 4 bits (both kernels, us, without / so.  Depth 256,
+  // bf16 and f16: one of 131055 keys 41.6 / 37.5, 70.3 / 61.4; 64 ragged ones 64.8 / 55.0, 94.8 / 81.0; 8 of 3000 18.8 / 19.1, 23.2 / 22.2; 320 key heads of
+  // 1024 keys of their own 72.2 / 55.8, 8 of 4096 14.7 / 15.8.  128 and 64, bf16: one of 131055 45.1 / 45.7, 30.5 / 32.5; 64 ragged ones 57.7 / 58.2, 40.1 /
+  // 41.9; 8 of 3000 14.7 / 16.1, 12.5 / 14.0).
   constexpr bool kPast = kFour && kDepth == 256;
   auto ask_pages = [&](int tile) {
     if (kPast) tile = min(tile, end - 1);

@@ -4,9 +4,11 @@
 // A number that bf16 does not have goes to the next one below or above, so the bounds stay bounds; elements that are no numbers have
 // no part.  Of each sequence the pages that hold its newest tokens are written, from the keys that it has there.
 //
-// Bound by the bytes of the keys: 5 sequences of 9001 to 32768 keys, 8 key heads of 128 in e4m3, pages of 64, 118 MB: 24.8 us, 4.8 TB/s (the
-// same with two, four and eight loads ahead; 38.7 with a block to a page, a thread to a channel 147); the page that each of 64
-// streams wrote to, 16 keys of 8 heads in bf16: 3.2 us, a launch.
+// 5 sequences of 9001 to 32768 keys, 8 key heads of 128 in e4m3, pages of 64, 118 MB: 24.8 us, 4.8 TB/s (the same with two, four and eight loads
+// ahead; 38.7 with a block to a page, a thread to a channel 147).  Bound by memory and the waves' own work, which overlap only
+// between waves (one asks for its vectors, folds them, asks again, and ends): of 103 MB in such pages, 22.7 us, a plain read of the same runs takes 16.3 (6.3
+// TB/s, in any order of pages and with or without the values between them) and the kernel over one page again and again 14.1 (in bf16
+// 39.4 and 27.8, in 4 bits 22.6 and 18.5).  The page that each of 64 streams wrote to, 16 keys of 8 heads in bf16: 3.2 us, a launch.
 #include <algorithm>
 
 #include "cache_types.h"

@@ -2,8 +2,8 @@
 //
 // A thread moves eight elements of a head (16 bytes of f16 / bf16), sixteen for a cache of e4m3 where the depth allows, or, where
 // a row is not made of whole aligned vectors, one; into 4 bits eight, four threads to a scale, or all 32 of a scale.  Bound by bytes: every element is read once and written once (8192 tokens of 8
-// heads of 128, bf16 to e4m3, 50 MB: 11.2 us, 4.5 TB/s where a large copy reaches 4.9; eight elements to a thread 14.1; 64 tokens
-// kept as bf16, 3.2 us, a launch).
+// heads of 128, bf16 to e4m3, 50 MB: 11.2 us, 4.5 TB/s where a large copy reaches 4.9; eight elements to a thread 14.1; to 4 bits,
+// 42 MB, 11.8, 3.6 TB/s; 64 tokens kept as bf16, 3.2 us, a launch; 1037 to 4 bits 3.1).
 // Threads, and so the vectors of a token, are in no order: a slot of several tokens holds a mix of their vectors (700 tokens of 8
 // heads of 128 to one slot: 97 of 100 launches).  To have one token win, each block would look through the tokens after its own:
 // 8192 tokens 14.9 us instead of 11.2, 65536 of one head 55 instead of 7; slots are a server's own and differ.

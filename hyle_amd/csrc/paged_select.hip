@@ -1,8 +1,10 @@
 // paged_select.hip -- the pages of each sequence that a query's products can be largest in, for every key head.
 //
 // score of a page = max over the key head's query heads and the new rows of sum_d q_d (q_d >= 0 ? high_d : low_d)
-// which no key of the page passes.  Sums are kept in 64 bits and rounded once to f32, so that the order of pages does not depend on
-// the order of additions; the products of f16 and bf16 numbers are exact.  A score that is no number counts as the largest.  The
+// which no key of the page passes.  Products are exact in 64 bits (11 or 24 bits by 8); sums are kept there and rounded once to f32.  The kernels
+// below add in orders of their own, which moves a sum by 2^-45 of its terms' magnitudes at most (256 of them): so two of them may give
+// neighbouring f32 numbers for a sum that lies so close to the middle between them, or whose terms cancel, and the choice differs where
+// that decides between two pages.  A score that is no number counts as the largest.  The
 // first page and those of the newest tokens are always chosen, then the best, ties to the earlier, and written in their order.
 // Two launches: scores to the workspace, and one block to a key head that finds the last chosen score digit by digit.
 //

@@ -7,8 +7,10 @@
 // the cache keeps.
 //
 // Bound by bytes: 8192 tokens of 32 query and 8 key heads of 128, bf16 to e4m3, 184 MB: 33.7 us, 5.5 TB/s (a wave to a row, which works out
-// its own cos and sin, 162); 64 tokens kept as bf16, 3.4 us, a launch; 1037 of 20 and 5 heads of 96 to 4 bits 6.7 us, launch, position,
-// 64-bit cos and sin, rows and LDS one after another (half and four times the waves: the same).
+// its own cos and sin, 162), to 4 bits 34.2; 64 tokens kept as bf16, 3.4 us, a launch; 1037 of 20 and 5 heads of 96 to 4 bits 6.7 us, launch, position,
+// 64-bit cos and sin, rows and LDS one after another (half and four times the waves: the same).  Depths and rotary widths that are no multiples of
+// 16 take a wave to a row: of the 8192 tokens, us as bf16 / e4m3 / 4 bits, width 128 37.3 / 34.3 / 34.2, 120 140 / 138 / 172, 40 162 / 157 / 197;
+// depth 80, width 80 31.8, 40 142 (64 tokens 3.3 and 3.6).
 #include "cache_types.h"
 
 namespace hyle_hip {
